@@ -338,6 +338,48 @@ typedef struct rg_sgd_args {
 } rg_sgd_args;
 int rg_sgd_step(rg_optim* opt, const rg_sgd_args* args, void* stream);
 
+/* ---------------------------------------------------------------- optimizer states in 8 bits */
+
+/* The two moments of Adam in 8 bits each: 4 bytes of state traffic per element and step instead of 16, 2 bytes of memory
+ * instead of 8.  No counterpart in the reference, which keeps torch.optim's fp32 states.
+ *
+ * Form.  A tensor's state is `numel` codes (one byte each, e4m3) and rg_state8_num_scales(numel) = ceil(numel / 256)
+ * fp32 scales, one for every 256 consecutive elements (the last block may be shorter).  A block's scale s is its largest
+ * magnitude; element x has the e4m3 number that 256 * x / s is rounded to, and reads back as code * (s / 256).  The second
+ * moment is held as its square root.  A block with s < 2^-100 holds zeros (s = 0); one in which anything is infinite or NaN
+ * has s = NaN and zero codes, so it reads back as NaN; a root that is not zero never gets the code of zero.
+ *
+ * rg_optim_create_state8 makes a table like rg_optim_create's whose states are in that form: codes1 / scales1 hold
+ * exp_avg, codes2 / scales2 the root of exp_avg_sq (all zero bytes before the first step).  Codes and scales must be
+ * 4-byte aligned.  rg_adam_step, rg_adam_step_clocked, rg_optim_set_grad_scale_source, rg_optim_update_pointers (with
+ * state1 = state2 = NULL: states stay where they are) and rg_optim_destroy take such a table; rg_sgd_step does not.
+ *
+ * Arithmetic of its Adam step, every operation in fp32 and rounded by itself (the division of the last line is within
+ * 2 units in the last place), with g, p and the scalar factors as for rg_adam_step:
+ *   m = beta1 * m + (1 - beta1) * g
+ *   v = beta2 * (r * r) + ((1 - beta2) * g) * g,   r = sqrt(v)
+ *   p = p + ((-lr / (1 - beta1^step)) * m) / (r * (1 / sqrt(1 - beta2^step)) + eps)
+ * The parameter sees m and r before they are rounded to 8 bits.  That rounding is dithered: with y = 256 * x / s and q the
+ * distance of the two e4m3 numbers around |y|, the code is floor(|y| / q + u / 2^20) * q with y's sign (|y| / q cut to
+ * multiples of 2^-20), u the upper 20 bits of i * 0xD1B54A33 + step * 0xABC98389 (exp_avg) or * 0x8CB92BA7 (the root)
+ * mod 2^32, i the element's place in its tensor.  The same inputs give the same bits on every run. */
+#define RG_STATE8_BLOCK 256
+int64_t rg_state8_num_scales(int64_t numel);   /* -1 for a negative count */
+int rg_optim_create_state8(rg_optim** out, int device, int n_tensors, void* const* param, const void* const* grad,
+                           void* const* codes1, float* const* scales1, void* const* codes2, float* const* scales2,
+                           void* const* model_copy, const int64_t* numel, const int* grad_dtype, const int* copy_dtype);
+
+/* The same form from and to fp32, many tensors in one launch (a checkpoint in 32 bits is loaded or written).
+ * root[i] != 0: values[i] is a second moment, stored as its root and read back as the root's square.  Quantizing
+ * rounds to nearest, ties to even; what dequantizing gives quantizes to the same codes and scales again (roots: as long as the
+ * squares are normal fp32 numbers).  A negative value under `root` counts as NaN.  The table borrows the addresses. */
+typedef struct rg_state8 rg_state8;
+int rg_state8_create(rg_state8** out, int device, int n_tensors, void* const* codes, float* const* scales, float* const* values,
+                     const int64_t* numel, const int* root);
+int rg_state8_quantize(rg_state8* table, void* stream);     /* values -> codes, scales */
+int rg_state8_dequantize(rg_state8* table, void* stream);   /* codes, scales -> values */
+int rg_state8_destroy(rg_state8* table);
+
 /* ---------------------------------------------------------------- loss scale on the device */
 
 /* The dynamic loss-scale schedule as a one-thread kernel, so that a mixed-precision step needs no host read:

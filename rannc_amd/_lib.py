@@ -83,6 +83,12 @@ SIGNATURES = {
     "rg_optim_create": (_i, [C.POINTER(_vp), _i, _i, _pvp, _pvp, _pvp, _pvp, _pvp, _pi64, _pi, _pi]),
     "rg_optim_update_pointers": (_i, [_vp, _pvp, _pvp, _pvp, _pvp, _pvp, _vp]),
     "rg_optim_destroy": (_i, [_vp]),
+    "rg_optim_create_state8": (_i, [C.POINTER(_vp), _i, _i, _pvp, _pvp, _pvp, _pvp, _pvp, _pvp, _pvp, _pi64, _pi, _pi]),
+    "rg_state8_num_scales": (_i64, [_i64]),
+    "rg_state8_create": (_i, [C.POINTER(_vp), _i, _i, _pvp, _pvp, _pvp, _pi64, _pi]),
+    "rg_state8_quantize": (_i, [_vp, _vp]),
+    "rg_state8_dequantize": (_i, [_vp, _vp]),
+    "rg_state8_destroy": (_i, [_vp]),
     "rg_adam_step": (_i, [_vp, C.POINTER(AdamArgs), _vp]),
     "rg_adam_step_clocked": (_i, [_vp, C.POINTER(AdamArgs), _vp, _vp]),
     "rg_adam_clock_advance": (_i, [_vp, C.c_double, C.c_double, C.c_double, _vp, _i, _vp]),
@@ -369,18 +375,68 @@ def adam_clock_advance(clock_ptr: int, lr: float, beta1: float, beta2: float, ga
     check(lib.rg_adam_clock_advance(_vp(clock_ptr), lr, beta1, beta2, _vp(gate or None), device, _vp(stream)))
 
 
+STATE8_BLOCK = 256     # elements of an 8-bit state that share a scale
+
+
+def state8_num_scales(numel: int) -> int:
+    n = lib.rg_state8_num_scales(numel)
+    if n < 0:
+        raise ValueError(f"negative element count {numel}")
+    return n
+
+
+class State8Table:
+    """Owner of one ``rg_state8``: addresses of 8-bit states and of the fp32 values they are converted from and to."""
+
+    def __init__(self, device: int, codes: Sequence[int], scales: Sequence[int], values: Sequence[int], numels: Sequence[int],
+                 roots: Sequence[bool]):
+        n = len(numels)
+        self._handle = _vp()
+        check(lib.rg_state8_create(C.byref(self._handle), device, n, _ptr_array(codes, n), _ptr_array(scales, n),
+                                   _ptr_array(values, n), (C.c_int64 * max(n, 1))(*numels), (C.c_int * max(n, 1))(*map(int, roots))))
+
+    def quantize(self, stream: int = 0) -> None:
+        check(lib.rg_state8_quantize(self._handle, _vp(stream)))
+
+    def dequantize(self, stream: int = 0) -> None:
+        check(lib.rg_state8_dequantize(self._handle, _vp(stream)))
+
+    def is_open(self) -> bool:
+        return bool(self._handle)
+
+    def close(self) -> None:
+        if self._handle:
+            lib.rg_state8_destroy(self._handle)
+            self._handle = _vp()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
 class OptimTable:
     """Owner of one ``rg_optim``: parameter / gradient / state / model-copy pointers of the
     tensors one optimizer launch updates."""
 
     def __init__(self, device: int, params: Sequence[int], grads: Sequence[int], state1: Optional[Sequence[int]],
                  state2: Optional[Sequence[int]], copies: Optional[Sequence[Optional[int]]], numels: Sequence[int],
-                 grad_dtypes: Sequence[int], copy_dtypes: Optional[Sequence[int]] = None):
+                 grad_dtypes: Sequence[int], copy_dtypes: Optional[Sequence[int]] = None,
+                 scales1: Optional[Sequence[int]] = None, scales2: Optional[Sequence[int]] = None):
+        """With ``scales1`` and ``scales2`` the states are in 8 bits: ``state1`` / ``state2`` are the codes of exp_avg
+        and of exp_avg_sq's root, and every 256 elements of a tensor have a float of each of the two."""
         n = len(numels)
         self._handle = _vp()
         self.n = n
         self.device = device
         a_cd = (C.c_int * max(n, 1))(*(copy_dtypes if copy_dtypes is not None else [RG_F32] * n))
+        if scales1 is not None or scales2 is not None:
+            check(lib.rg_optim_create_state8(C.byref(self._handle), device, n, _ptr_array(params, n), _ptr_array(grads, n),
+                                             _ptr_array(state1, n), _ptr_array(scales1, n), _ptr_array(state2, n),
+                                             _ptr_array(scales2, n), _ptr_array(copies, n),
+                                             (C.c_int64 * max(n, 1))(*numels), (C.c_int * max(n, 1))(*grad_dtypes), a_cd))
+            return
         check(lib.rg_optim_create(C.byref(self._handle), device, n, _ptr_array(params, n), _ptr_array(grads, n),
                                   _ptr_array(state1, n), _ptr_array(state2, n), _ptr_array(copies, n),
                                   (C.c_int64 * max(n, 1))(*numels), (C.c_int * max(n, 1))(*grad_dtypes), a_cd))

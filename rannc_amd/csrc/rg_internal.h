@@ -181,6 +181,51 @@ hipError_t launch_reduce(const ReduceArgs& a, int64_t n_chunks, hipStream_t stre
 // segment sums (left by an earlier launch_reduce) -> per-tensor norms -> decision for a.max_norm
 hipError_t launch_decide(const ReduceArgs& a, hipStream_t stream);
 hipError_t launch_fill_zero(void* dst, int64_t nbytes, hipStream_t stream);
+
+// ---- optimizer states in 8 bits (rg_state8.hip)
+
+constexpr int64_t kMaxTensorElems = (int64_t)1 << 44;   // 16 TiB of codes: keeps the sums of sizes far from overflow
+constexpr int kState8Block = RG_STATE8_BLOCK;   // elements that share a scale
+
+// One row of the work table of an optimizer step with 8-bit states: a run of whole blocks of one parameter (the last
+// block may be shorter).
+struct Opt8ChunkRec {
+  void* param;
+  const void* grad;
+  void* codes1;
+  float* scales1;
+  void* codes2;
+  float* scales2;
+  void* copy;
+  int32_t len;
+  uint32_t first;        // the run's first element in its tensor, mod 2^32
+  int16_t grad_dtype;
+  int16_t copy_dtype;
+  int32_t pad[3];
+};
+static_assert(sizeof(Opt8ChunkRec) == 80, "8-bit optimizer chunk record must stay 80 bytes");
+
+// Scalar factors of the Adam step, rounded once from double on the host.
+struct Adam8Const {
+  float grad_scale;        // negative: maximize
+  float weight_decay;      // L2 form: g += wd * p (0 = off)
+  float param_mul;         // decoupled form: p *= 1 - lr * wd (1 = off)
+  float beta1, one_minus_beta1, beta2, one_minus_beta2;
+  float neg_step_size, inv_bias2_sqrt, eps;
+};
+
+struct Adam8Args {
+  const Opt8ChunkRec* chunks;
+  const StepResult* gate;
+  const rg_adam_clock* clock;   // optional: the step count and the factors that depend on it live on the device
+  const float* grad_scale_dev;  // optional: the gradient scale lives on the device
+  float grad_scale_sign;        // ... and is multiplied by this (-1: maximize)
+  uint32_t step;
+  int32_t tiles_per_chunk;
+  Adam8Const c;
+};
+
+hipError_t launch_adam8(const Adam8Args& a, int64_t n_chunks, int64_t chunk_elems, bool streaming, hipStream_t stream);
 // Ticks of the current device's wall clock that a wavefront of a large flat fill waits before it stores (0: unknown rate).
 int fill_delay_ticks();
 int fill_delay_ticks(int ns);   // the same clock, another delay

@@ -9,6 +9,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <memory>
 #include <new>
 #include <vector>
 
@@ -299,20 +300,24 @@ struct rg_optim {
   int64_t chunk_elems = RG_DEFAULT_CHUNK_ELEMS;
   int64_t total_numel = 0;
   bool has_state1 = false, has_state2 = false, any_copy = false;
+  bool state8 = false;                     // states in 8 bits: state1 / state2 are codes, scale1 / scale2 their blocks' scales
   const float* grad_scale_dev = nullptr;   // rg_optim_set_grad_scale_source
   struct Row {
     void* param;
     const void* grad;
     void* state1;
     void* state2;
+    float* scale1;
+    float* scale2;
     void* copy;
     int64_t numel;
     int32_t grad_dtype, copy_dtype;
   };
   std::vector<Row> rows;
   std::vector<int64_t> chunk_begin;
-  OptChunkRec* d_chunks = nullptr;
-  OptChunkRec* stage[2] = {nullptr, nullptr};   // pinned
+  size_t table_bytes() const { return (size_t)n_chunks * (state8 ? sizeof(Opt8ChunkRec) : sizeof(OptChunkRec)); }
+  void* d_chunks = nullptr;                // OptChunkRec[n_chunks], or Opt8ChunkRec[n_chunks]
+  void* stage[2] = {nullptr, nullptr};     // pinned
   hipEvent_t stage_done[2] = {nullptr, nullptr};
   bool stage_used[2] = {false, false};
   int next_stage = 0;
@@ -341,6 +346,35 @@ static void fill_opt_records(const rg_optim* o, OptChunkRec* out) {
   }
 }
 
+// Chunks of a table with 8-bit states hold whole blocks, so they are counted from the tensor's first element.
+static void fill_opt8_records(const rg_optim* o, Opt8ChunkRec* out) {
+  for (int i = 0; i < o->n_tensors; ++i) {
+    const rg_optim::Row& t = o->rows[(size_t)i];
+    const int gs = elem_size(t.grad_dtype), cs = elem_size(t.copy_dtype);
+    for (int64_t c = o->chunk_begin[(size_t)i]; c < o->chunk_begin[(size_t)i + 1]; ++c) {
+      const int64_t start = (c - o->chunk_begin[(size_t)i]) * o->chunk_elems;
+      Opt8ChunkRec& r = out[c];
+      memset(&r, 0, sizeof(r));
+      r.param = static_cast<char*>(t.param) + start * 4;
+      r.grad = static_cast<const char*>(t.grad) + start * gs;
+      r.codes1 = static_cast<char*>(t.state1) + start;
+      r.scales1 = t.scale1 + start / kState8Block;
+      r.codes2 = static_cast<char*>(t.state2) + start;
+      r.scales2 = t.scale2 + start / kState8Block;
+      r.copy = t.copy ? static_cast<char*>(t.copy) + start * cs : nullptr;
+      r.len = (int32_t)std::min(t.numel - start, o->chunk_elems);
+      r.first = (uint32_t)start;
+      r.grad_dtype = (int16_t)t.grad_dtype;
+      r.copy_dtype = (int16_t)t.copy_dtype;
+    }
+  }
+}
+
+static void fill_table(const rg_optim* o, void* out) {
+  if (o->state8) fill_opt8_records(o, static_cast<Opt8ChunkRec*>(out));
+  else fill_opt_records(o, static_cast<OptChunkRec*>(out));
+}
+
 static int check_rows(const rg_optim* o, const char* op) {
   for (int i = 0; i < o->n_tensors; ++i) {
     const rg_optim::Row& t = o->rows[(size_t)i];
@@ -355,83 +389,118 @@ static int check_rows(const rg_optim* o, const char* op) {
     }
     int rc = check_pointer(t.param, 4, "param", i);
     if (rc == RG_OK) rc = check_pointer(t.grad, elem_size(t.grad_dtype), "grad", i);
+    // codes are read four at a time, so they need the alignment of fp32 states too
     if (rc == RG_OK) rc = check_pointer(t.state1, 4, "state1", i);
     if (rc == RG_OK) rc = check_pointer(t.state2, 4, "state2", i);
     if (rc == RG_OK) rc = check_pointer(t.copy, elem_size(t.copy_dtype), "model_copy", i);
+    if (rc == RG_OK) rc = check_pointer(t.scale1, 4, "scale1", i);
+    if (rc == RG_OK) rc = check_pointer(t.scale2, 4, "scale2", i);
     if (rc != RG_OK) return rc;
+    if (o->state8 && (t.scale1 == nullptr || t.scale2 == nullptr)) {
+      set_error("%s: tensor %d lacks its scales", op, i);
+      return RG_EINVAL;
+    }
   }
   return RG_OK;
 }
 
-RG_API int rg_optim_create(rg_optim** out, int device, int n, void* const* param, const void* const* grad,
-                           void* const* state1, void* const* state2, void* const* model_copy, const int64_t* numel,
-                           const int* grad_dtype, const int* copy_dtype) {
-  if (out == nullptr || n < 0 || (n > 0 && (param == nullptr || grad == nullptr || numel == nullptr || grad_dtype == nullptr))) {
-    set_error("rg_optim_create: bad arguments");
+struct OptColumns {
+  void* const* param;
+  const void* const* grad;
+  void* const* state1;
+  void* const* state2;
+  float* const* scale1;
+  float* const* scale2;
+  void* const* model_copy;
+  const int64_t* numel;
+  const int* grad_dtype;
+  const int* copy_dtype;
+};
+
+static int create_table(rg_optim** out, int device, int n, const OptColumns& a, bool state8, const char* op) try {
+  if (out == nullptr || n < 0 ||
+      (n > 0 && (a.param == nullptr || a.grad == nullptr || a.numel == nullptr || a.grad_dtype == nullptr)) ||
+      (n > 0 && state8 && (a.state1 == nullptr || a.state2 == nullptr || a.scale1 == nullptr || a.scale2 == nullptr))) {
+    set_error("%s: bad arguments", op);
     return RG_EINVAL;
   }
   *out = nullptr;
-  rg_optim* o = new (std::nothrow) rg_optim;
-  if (o == nullptr) {
-    set_error("rg_optim_create: out of host memory");
-    return RG_ENOMEM;
-  }
+  struct Destroy {
+    void operator()(rg_optim* t) const { (void)rg_optim_destroy(t); }
+  };
+  std::unique_ptr<rg_optim, Destroy> owner(new rg_optim);
+  rg_optim* o = owner.get();
   o->device = device;
   o->n_tensors = n;
-  o->has_state1 = state1 != nullptr;
-  o->has_state2 = state2 != nullptr;
+  o->state8 = state8;
+  o->has_state1 = state8 || a.state1 != nullptr;
+  o->has_state2 = state8 || a.state2 != nullptr;
   o->rows.resize((size_t)n);
   o->chunk_begin.assign((size_t)n + 1, 0);
   for (int i = 0; i < n; ++i) {
     rg_optim::Row& t = o->rows[(size_t)i];
-    t.param = param[i];
-    t.grad = grad[i];
-    t.state1 = state1 ? state1[i] : nullptr;
-    t.state2 = state2 ? state2[i] : nullptr;
-    t.copy = model_copy ? model_copy[i] : nullptr;
-    t.numel = numel[i];
-    t.grad_dtype = grad_dtype[i];
-    t.copy_dtype = (model_copy && model_copy[i] && copy_dtype) ? copy_dtype[i] : RG_F32;
+    t.param = a.param[i];
+    t.grad = a.grad[i];
+    t.state1 = a.state1 ? a.state1[i] : nullptr;
+    t.state2 = a.state2 ? a.state2[i] : nullptr;
+    t.scale1 = a.scale1 ? a.scale1[i] : nullptr;
+    t.scale2 = a.scale2 ? a.scale2[i] : nullptr;
+    t.copy = a.model_copy ? a.model_copy[i] : nullptr;
+    t.numel = a.numel[i];
+    t.grad_dtype = a.grad_dtype[i];
+    t.copy_dtype = (a.model_copy && a.model_copy[i] && a.copy_dtype) ? a.copy_dtype[i] : RG_F32;
     if (t.copy) o->any_copy = true;
-    if (t.numel < 0 || elem_size(t.grad_dtype) < 0 || elem_size(t.copy_dtype) < 0) {
-      set_error("rg_optim_create: tensor %d has a bad size or dtype", i);
-      delete o;
+    if (t.numel < 0 || t.numel > kMaxTensorElems || elem_size(t.grad_dtype) < 0 || elem_size(t.copy_dtype) < 0) {
+      set_error("%s: tensor %d has a bad size or dtype", op, i);
       return RG_EINVAL;
     }
     o->total_numel += t.numel;
     o->chunk_begin[(size_t)i + 1] = o->chunk_begin[(size_t)i] + (t.numel + o->chunk_elems - 1) / o->chunk_elems;
   }
   o->n_chunks = o->chunk_begin[(size_t)n];
-  int rc = check_rows(o, "rg_optim_create");
+  int rc = check_rows(o, op);
   const int64_t tiles = (o->chunk_elems + kOptMinTileElems - 1) / kOptMinTileElems;
   if (rc == RG_OK && o->n_chunks * tiles > 0x7fffffffLL) {
-    set_error("rg_optim_create: %lld elements exceed one launch", (long long)o->total_numel);
+    set_error("%s: %lld elements exceed one launch", op, (long long)o->total_numel);
     rc = RG_EINVAL;
   }
-  if (rc != RG_OK) {
-    delete o;
-    return rc;
-  }
+  if (rc != RG_OK) return rc;
   if (o->n_chunks > 0) {
     DeviceGuard guard(device);
-    const size_t bytes = (size_t)o->n_chunks * sizeof(OptChunkRec);
-    hipError_t e = hipMalloc(reinterpret_cast<void**>(&o->d_chunks), bytes);
+    const size_t bytes = o->table_bytes();
+    hipError_t e = hipMalloc(&o->d_chunks, bytes);
     for (int k = 0; k < 2 && e == hipSuccess; ++k) {
-      e = hipHostMalloc(reinterpret_cast<void**>(&o->stage[k]), bytes, hipHostMallocDefault);
+      e = hipHostMalloc(&o->stage[k], bytes, hipHostMallocDefault);
       if (e == hipSuccess) e = hipEventCreateWithFlags(&o->stage_done[k], hipEventDisableTiming);
     }
     if (e == hipSuccess) {
-      fill_opt_records(o, o->stage[0]);
+      fill_table(o, o->stage[0]);
       e = hipMemcpy(o->d_chunks, o->stage[0], bytes, hipMemcpyHostToDevice);
     }
     if (e != hipSuccess) {
-      const int code = hip_fail(e, "rg_optim_create");
-      (void)rg_optim_destroy(o);
+      const int code = hip_fail(e, op);
       return e == hipErrorOutOfMemory ? RG_ENOMEM : code;
     }
   }
-  *out = o;
+  *out = owner.release();
   return RG_OK;
+} catch (const std::bad_alloc&) {
+  set_error("%s: out of host memory", op);
+  return RG_ENOMEM;
+}
+
+RG_API int rg_optim_create(rg_optim** out, int device, int n, void* const* param, const void* const* grad,
+                           void* const* state1, void* const* state2, void* const* model_copy, const int64_t* numel,
+                           const int* grad_dtype, const int* copy_dtype) {
+  const OptColumns a = {param, grad, state1, state2, nullptr, nullptr, model_copy, numel, grad_dtype, copy_dtype};
+  return create_table(out, device, n, a, false, "rg_optim_create");
+}
+
+RG_API int rg_optim_create_state8(rg_optim** out, int device, int n, void* const* param, const void* const* grad,
+                                  void* const* codes1, float* const* scales1, void* const* codes2, float* const* scales2,
+                                  void* const* model_copy, const int64_t* numel, const int* grad_dtype, const int* copy_dtype) {
+  const OptColumns a = {param, grad, codes1, codes2, scales1, scales2, model_copy, numel, grad_dtype, copy_dtype};
+  return create_table(out, device, n, a, true, "rg_optim_create_state8");
 }
 
 RG_API int rg_optim_destroy(rg_optim* o) {
@@ -459,6 +528,10 @@ RG_API int rg_optim_update_pointers(rg_optim* o, void* const* param, const void*
     set_error("rg_optim_update_pointers: the table was created without these state arrays");
     return RG_EINVAL;
   }
+  if (o->state8 && (state1 != nullptr || state2 != nullptr)) {
+    set_error("rg_optim_update_pointers: the states of a table created with 8-bit states stay where they are");
+    return RG_EINVAL;
+  }
   std::vector<rg_optim::Row> saved = o->rows;
   for (int i = 0; i < o->n_tensors; ++i) {
     rg_optim::Row& t = o->rows[(size_t)i];
@@ -483,9 +556,9 @@ RG_API int rg_optim_update_pointers(rg_optim* o, void* const* param, const void*
   const int k = o->next_stage;
   o->next_stage ^= 1;
   if (o->stage_used[k]) RG_HIP(hipEventSynchronize(o->stage_done[k]));
-  fill_opt_records(o, o->stage[k]);
+  fill_table(o, o->stage[k]);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  RG_HIP(hipMemcpyAsync(o->d_chunks, o->stage[k], (size_t)o->n_chunks * sizeof(OptChunkRec), hipMemcpyHostToDevice, s));
+  RG_HIP(hipMemcpyAsync(o->d_chunks, o->stage[k], o->table_bytes(), hipMemcpyHostToDevice, s));
   RG_HIP(hipEventRecord(o->stage_done[k], s));
   o->stage_used[k] = true;
   return RG_OK;
@@ -498,7 +571,7 @@ static int launch_optim(const rg_optim* o, const OptConst& c, const rg_step_resu
   DeviceGuard guard(o->device);
   OptArgs a;
   memset(&a, 0, sizeof(a));
-  a.chunks = o->d_chunks;
+  a.chunks = static_cast<const OptChunkRec*>(o->d_chunks);
   a.gate = reinterpret_cast<const StepResult*>(gate);
   a.clock = clock;
   a.grad_scale_dev = o->grad_scale_dev;
@@ -536,6 +609,31 @@ static int adam_step(rg_optim* o, const rg_adam_args* g, const rg_adam_clock* cl
   // The scalar factors as torch/optim/adam.py computes them: in double, from Python floats.
   const double bias1 = 1.0 - pow(g->beta1, (double)step);
   const double bias2 = 1.0 - pow(g->beta2, (double)step);
+  if (o->state8) {
+    if (o->n_chunks == 0) return RG_OK;
+    Adam8Args a;
+    memset(&a, 0, sizeof(a));
+    a.chunks = static_cast<const Opt8ChunkRec*>(o->d_chunks);
+    a.gate = reinterpret_cast<const StepResult*>(g->gate);
+    a.clock = clock;
+    a.grad_scale_dev = o->grad_scale_dev;
+    a.grad_scale_sign = g->maximize ? -1.0f : 1.0f;
+    a.step = (uint32_t)step;
+    a.c.grad_scale = g->maximize ? -g->grad_scale : g->grad_scale;
+    a.c.weight_decay = g->decoupled_weight_decay ? 0.0f : (float)g->weight_decay;
+    a.c.param_mul = g->decoupled_weight_decay ? (float)(1.0 - g->lr * g->weight_decay) : 1.0f;
+    a.c.beta1 = (float)g->beta1;
+    a.c.one_minus_beta1 = (float)(1.0 - g->beta1);
+    a.c.beta2 = (float)g->beta2;
+    a.c.one_minus_beta2 = (float)(1.0 - g->beta2);
+    a.c.neg_step_size = (float)(-(g->lr / bias1));
+    a.c.inv_bias2_sqrt = 1.0f / (float)sqrt(bias2);
+    a.c.eps = (float)g->eps;
+    DeviceGuard guard(o->device);
+    RG_HIP(launch_adam8(a, o->n_chunks, o->chunk_elems, o->total_numel * 18 > ((int64_t)256 << 20),
+                        reinterpret_cast<hipStream_t>(stream)));
+    return RG_OK;
+  }
   const double weight = 1.0 - g->beta1;
   OptConst c;
   memset(&c, 0, sizeof(c));
@@ -594,6 +692,10 @@ RG_API int rg_adam_clock_advance(rg_adam_clock* clock_dev, double lr, double bet
 RG_API int rg_sgd_step(rg_optim* o, const rg_sgd_args* g, void* stream) {
   if (o == nullptr || g == nullptr) {
     set_error("rg_sgd_step: null argument");
+    return RG_EINVAL;
+  }
+  if (o->state8) {
+    set_error("rg_sgd_step: the table was created with 8-bit states, which only the Adam step keeps");
     return RG_EINVAL;
   }
   if (!(g->lr >= 0.0) || !(g->momentum >= 0.0) || !(g->weight_decay >= 0.0) ||

@@ -1,0 +1,361 @@
+// Optimizer states in 8 bits: the Adam step that keeps both moments that way, and the conversions between 8 and 32 bits.
+#include <math.h>
+#include <string.h>
+
+#include <algorithm>
+#include <new>
+#include <vector>
+
+#include "rg_host.h"
+#include "rg_internal.h"
+#include "rg_state8.h"
+
+namespace rg {
+namespace {
+
+constexpr int kLaneElems = 4;                                   // elements of a block one lane holds: 64 lanes, 256 elements
+constexpr int kAdam8Threads = 256, kAdam8TileElems = 4096;      // 4 wavefronts, 4 blocks each
+constexpr int kConvThreads = 256, kConvTileElems = 4096;
+
+template <int DT> __device__ __forceinline__ float load_one(const char* p) { return __uint_as_float(load_u32(p)); }
+template <> __device__ __forceinline__ float load_one<RG_F16>(const char* p) {
+  return f16_to_f32(__builtin_bit_cast(_Float16, (unsigned short)load_u16(p)));
+}
+template <> __device__ __forceinline__ float load_one<RG_BF16>(const char* p) { return bf16_bits_to_f32(load_u16(p)); }
+
+// Four elements of a lane, of which `n` exist (the rest read as zeros).
+template <int DT, bool NT> __device__ __forceinline__ void load4(const char* p, int n, float (&f)[4]) {
+  if (n >= 4) {
+    Codec<DT, 4>::unpack(Mem<DT, 4, NT>::load(p), f);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f[j] = j < n ? load_one<DT>(p + (size_t)j * ElemSize<DT>::value) : 0.0f;
+}
+template <int DT, bool NT> __device__ __forceinline__ void store4(char* p, int n, const float (&f)[4]) {
+  if (n >= 4) {
+    Mem<DT, 4, NT>::store(p, Codec<DT, 4>::pack(f));
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (j < n) store1<DT>(p + (size_t)j * ElemSize<DT>::value, f[j]);
+}
+template <bool NT> __device__ __forceinline__ uint32_t load_codes4(const char* p, int n) {
+  if (n >= 4) return ld_codes<NT>(p);
+  uint32_t w = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (j < n) w |= load_u8(p + j) << (8 * j);
+  return w;
+}
+template <bool NT> __device__ __forceinline__ void store_codes4(char* p, int n, uint32_t w) {
+  if (n >= 4) {
+    st_codes<NT>(p, w);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (j < n) store_u8(p + j, (w >> (8 * j)) & 0xffu);
+}
+
+// One block of 256 elements (fewer at a tensor's end) by one wavefront.
+template <int G, int C, bool NT>
+__device__ __forceinline__ void adam8_block(const Opt8ChunkRec& r, int start, int lane, const Adam8Const& c, float coef,
+                                            uint32_t step) {
+  const int e = start + lane * kLaneElems;
+  const int n = r.len - e;                 // <= 0: this lane has no element
+  constexpr int CD = C >= 0 ? C : RG_F32;
+  char* pp = reinterpret_cast<char*>(r.param) + (ptrdiff_t)e * 4;
+  const char* gp = reinterpret_cast<const char*>(r.grad) + (ptrdiff_t)e * ElemSize<G>::value;
+  char* c1 = reinterpret_cast<char*>(r.codes1) + e;
+  char* c2 = reinterpret_cast<char*>(r.codes2) + e;
+  const int block = start / kState8Block;
+  float p[4], g[4], m[4], v[4];
+  load4<RG_F32, NT>(pp, n, p);
+  load4<G, NT>(gp, n, g);
+  const uint32_t w1 = load_codes4<NT>(c1, n), w2 = load_codes4<NT>(c2, n);
+  const float k1 = __uint_as_float(load_u32(reinterpret_cast<const char*>(r.scales1 + block))) * 0.00390625f;
+  const float k2 = __uint_as_float(load_u32(reinterpret_cast<const char*>(r.scales2 + block))) * 0.00390625f;
+  decode(w1, k1, m);
+  decode(w2, k2, v);
+  float root[4];
+  uint32_t top1 = 0, top2 = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float gj = g[j] * c.grad_scale;
+    gj = gj * coef;
+    p[j] = p[j] * c.param_mul;
+    if (c.weight_decay != 0.0f) gj = gj + c.weight_decay * p[j];
+    m[j] = c.beta1 * m[j] + c.one_minus_beta1 * gj;
+    const float vj = c.beta2 * (v[j] * v[j]) + (c.one_minus_beta2 * gj) * gj;
+    root[j] = sqrtf(vj);
+    p[j] = p[j] + (c.neg_step_size * m[j]) / (root[j] * c.inv_bias2_sqrt + c.eps);
+    const uint32_t a = magnitude_bits(m[j]), b = magnitude_bits(root[j]);
+    top1 = top1 > a ? top1 : a;
+    top2 = top2 > b ? top2 : b;
+  }
+  const BlockScale s1 = block_scale(wave_max(top1)), s2 = block_scale(wave_max(top2));
+  const uint32_t place = (r.first + (uint32_t)e) * kDitherPlace;
+  uint32_t o1 = 0, o2 = 0;
+  float y[4];
+  if (s1.inv != 0.0f) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = to_range<false>(m[j], s1.inv);
+    o1 = encode_dithered(y, place + step * kDitherFirst);
+  }
+  if (s2.inv != 0.0f) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = to_range<true>(root[j], s2.inv);
+    o2 = encode_dithered(y, place + step * kDitherRoot);
+  }
+  store4<RG_F32, NT>(pp, n, p);
+  if (C >= 0) store4<CD, NT>(reinterpret_cast<char*>(r.copy) + (ptrdiff_t)e * ElemSize<CD>::value, n, p);
+  store_codes4<NT>(c1, n, o1);
+  store_codes4<NT>(c2, n, o2);
+  if (lane == 0) {
+    store_u32(reinterpret_cast<char*>(r.scales1 + block), __float_as_uint(s1.s));
+    store_u32(reinterpret_cast<char*>(r.scales2 + block), __float_as_uint(s2.s));
+  }
+}
+
+template <bool NT>
+__global__ __launch_bounds__(kAdam8Threads) void adam8_kernel(Adam8Args a) {
+  float coef = 1.0f;
+  if (a.gate != nullptr) {
+    if (a.gate->skipped != 0) return;
+    coef = a.gate->coef;
+  }
+  if (a.grad_scale_dev != nullptr) a.c.grad_scale = a.grad_scale_sign * *a.grad_scale_dev;
+  uint32_t step = a.step;
+  if (a.clock != nullptr) {      // written by adam_clock_kernel earlier on the same stream
+    step = (uint32_t)a.clock->step;
+    a.c.neg_step_size = a.clock->neg_step_size;
+    a.c.inv_bias2_sqrt = 1.0f / a.clock->bias2_sqrt;
+  }
+  const unsigned bid = blockIdx.x;
+  const Opt8ChunkRec r = a.chunks[bid / (unsigned)a.tiles_per_chunk];
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64u)), lane = (int)(threadIdx.x % 64u);
+  constexpr int kWaveElems = kAdam8TileElems / (kAdam8Threads / 64);
+  const int start = (int)(bid % (unsigned)a.tiles_per_chunk) * kAdam8TileElems + wave * kWaveElems;
+  const int copy_kind = r.copy ? r.copy_dtype : -1;
+#define RG_ADAM8(G, C)                                                                                  \
+  if (r.grad_dtype == G && copy_kind == C) {                                                            \
+    for (int b = start; b < start + kWaveElems && b < r.len; b += kState8Block)                         \
+      adam8_block<G, C, NT>(r, b, lane, a.c, coef, step);                                               \
+    return;                                                                                             \
+  }
+  RG_ADAM8(RG_F32, -1)
+  RG_ADAM8(RG_F32, RG_BF16)
+  RG_ADAM8(RG_F32, RG_F16)
+  RG_ADAM8(RG_F32, RG_F32)
+  RG_ADAM8(RG_BF16, -1)
+  RG_ADAM8(RG_BF16, RG_BF16)
+  RG_ADAM8(RG_BF16, RG_F16)
+  RG_ADAM8(RG_BF16, RG_F32)
+  RG_ADAM8(RG_F16, -1)
+  RG_ADAM8(RG_F16, RG_F16)
+  RG_ADAM8(RG_F16, RG_BF16)
+  RG_ADAM8(RG_F16, RG_F32)
+#undef RG_ADAM8
+}
+
+// ---------------------------------------------------------------- conversions
+
+// One row of a conversion's work table: a run of whole blocks of one tensor (the last may be shorter).
+struct State8Rec {
+  void* codes;
+  float* scales;
+  float* values;
+  int32_t len;
+  int32_t root;
+};
+static_assert(sizeof(State8Rec) == 32, "conversion record must stay 32 bytes");
+
+template <bool ROOT, bool NT>
+__device__ __forceinline__ void quantize_block(const State8Rec& r, int start, int lane) {
+  const int e = start + lane * kLaneElems;
+  const int n = r.len - e;
+  float x[4];
+  load4<RG_F32, NT>(reinterpret_cast<const char*>(r.values) + (ptrdiff_t)e * 4, n, x);
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (ROOT) x[j] = sqrtf(x[j]);
+    const uint32_t a = magnitude_bits(x[j]);
+    top = top > a ? top : a;
+  }
+  const BlockScale s = block_scale(wave_max(top));
+  uint32_t w = 0;
+  if (s.inv != 0.0f) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = to_range<ROOT>(x[j], s.inv);
+    w = encode_nearest(x);
+  }
+  store_codes4<NT>(reinterpret_cast<char*>(r.codes) + e, n, w);
+  if (lane == 0) store_u32(reinterpret_cast<char*>(r.scales + start / kState8Block), __float_as_uint(s.s));
+}
+
+template <bool ROOT, bool NT>
+__device__ __forceinline__ void dequantize_block(const State8Rec& r, int start, int lane) {
+  const int e = start + lane * kLaneElems;
+  const int n = r.len - e;
+  const float k = __uint_as_float(load_u32(reinterpret_cast<const char*>(r.scales + start / kState8Block))) * 0.00390625f;
+  float x[4];
+  decode(load_codes4<NT>(reinterpret_cast<const char*>(r.codes) + e, n), k, x);
+  if (ROOT) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = x[j] * x[j];
+  }
+  store4<RG_F32, NT>(reinterpret_cast<char*>(r.values) + (ptrdiff_t)e * 4, n, x);
+}
+
+template <bool WRITE_CODES, bool NT>
+__global__ __launch_bounds__(kConvThreads) void state8_kernel(const State8Rec* recs, int tiles_per_chunk) {
+  const State8Rec r = recs[blockIdx.x / (unsigned)tiles_per_chunk];
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64u)), lane = (int)(threadIdx.x % 64u);
+  constexpr int kWaveElems = kConvTileElems / (kConvThreads / 64);
+  const int start = (int)(blockIdx.x % (unsigned)tiles_per_chunk) * kConvTileElems + wave * kWaveElems;
+  for (int b = start; b < start + kWaveElems && b < r.len; b += kState8Block) {
+    if (WRITE_CODES) {
+      if (r.root) quantize_block<true, NT>(r, b, lane);
+      else quantize_block<false, NT>(r, b, lane);
+    } else {
+      if (r.root) dequantize_block<true, NT>(r, b, lane);
+      else dequantize_block<false, NT>(r, b, lane);
+    }
+  }
+}
+
+}  // namespace
+
+hipError_t launch_adam8(const Adam8Args& args, int64_t n_chunks, int64_t chunk_elems, bool streaming, hipStream_t stream) {
+  Adam8Args a = args;
+  a.tiles_per_chunk = (int32_t)((chunk_elems + kAdam8TileElems - 1) / kAdam8TileElems);
+  const dim3 grid((unsigned)(n_chunks * a.tiles_per_chunk)), block(kAdam8Threads);
+  if (streaming) hipLaunchKernelGGL((adam8_kernel<true>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((adam8_kernel<false>), grid, block, 0, stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace rg
+
+using namespace rg;
+
+struct rg_state8 {
+  int device = 0;
+  int64_t n_chunks = 0;
+  int64_t total_numel = 0;
+  State8Rec* d_recs = nullptr;
+};
+
+constexpr int64_t kState8ChunkElems = 16384;
+
+RG_API int64_t rg_state8_num_scales(int64_t numel) { return numel < 0 ? -1 : (numel + kState8Block - 1) / kState8Block; }
+
+RG_API int rg_state8_create(rg_state8** out, int device, int n, void* const* codes, float* const* scales, float* const* values,
+                            const int64_t* numel, const int* root) {
+  if (out == nullptr || n < 0 ||
+      (n > 0 && (codes == nullptr || scales == nullptr || values == nullptr || numel == nullptr || root == nullptr))) {
+    set_error("rg_state8_create: bad arguments");
+    return RG_EINVAL;
+  }
+  *out = nullptr;
+  int64_t chunks = 0, total = 0;
+  for (int i = 0; i < n; ++i) {
+    if (numel[i] < 0) {
+      set_error("rg_state8_create: tensor %d has a negative size", i);
+      return RG_EINVAL;
+    }
+    if (numel[i] == 0) continue;
+    if (codes[i] == nullptr || scales[i] == nullptr || values[i] == nullptr) {
+      set_error("rg_state8_create: tensor %d lacks its codes, scales or values", i);
+      return RG_EINVAL;
+    }
+    int rc = check_pointer(codes[i], 4, "codes", i);
+    if (rc == RG_OK) rc = check_pointer(scales[i], 4, "scales", i);
+    if (rc == RG_OK) rc = check_pointer(values[i], 4, "values", i);
+    if (rc != RG_OK) return rc;
+    if (numel[i] > kMaxTensorElems) {
+      set_error("rg_state8_create: tensor %d has %lld elements", i, (long long)numel[i]);
+      return RG_EINVAL;
+    }
+    chunks += (numel[i] + kState8ChunkElems - 1) / kState8ChunkElems;
+    total += numel[i];
+    if (chunks * (kState8ChunkElems / kConvTileElems) > 0x7fffffffLL) {
+      set_error("rg_state8_create: %lld elements exceed one launch", (long long)total);
+      return RG_EINVAL;
+    }
+  }
+  rg_state8* t = new (std::nothrow) rg_state8;
+  if (t == nullptr) {
+    set_error("rg_state8_create: out of host memory");
+    return RG_ENOMEM;
+  }
+  t->device = device;
+  t->n_chunks = chunks;
+  t->total_numel = total;
+  if (chunks > 0) {
+    State8Rec* recs = new (std::nothrow) State8Rec[(size_t)chunks];
+    if (recs == nullptr) {
+      delete t;
+      set_error("rg_state8_create: out of host memory");
+      return RG_ENOMEM;
+    }
+    int64_t c = 0;
+    for (int i = 0; i < n; ++i) {
+      for (int64_t start = 0; start < numel[i]; start += kState8ChunkElems, ++c) {
+        State8Rec& r = recs[c];
+        r.codes = static_cast<char*>(codes[i]) + start;
+        r.scales = scales[i] + start / kState8Block;
+        r.values = values[i] + start;
+        r.len = (int32_t)std::min(numel[i] - start, kState8ChunkElems);
+        r.root = root[i] ? 1 : 0;
+      }
+    }
+    DeviceGuard guard(device);
+    hipError_t e = hipMalloc(reinterpret_cast<void**>(&t->d_recs), (size_t)chunks * sizeof(State8Rec));
+    if (e == hipSuccess) e = hipMemcpy(t->d_recs, recs, (size_t)chunks * sizeof(State8Rec), hipMemcpyHostToDevice);
+    delete[] recs;
+    if (e != hipSuccess) {
+      const int code = hip_fail(e, "rg_state8_create");
+      (void)rg_state8_destroy(t);
+      return e == hipErrorOutOfMemory ? RG_ENOMEM : code;
+    }
+  }
+  *out = t;
+  return RG_OK;
+}
+
+RG_API int rg_state8_destroy(rg_state8* t) {
+  if (t == nullptr) return RG_OK;
+  DeviceGuard guard(t->device);
+  if (t->d_recs) (void)hipFree(t->d_recs);
+  delete t;
+  return RG_OK;
+}
+
+static int launch_state8(const rg_state8* t, bool write_codes, void* stream, const char* op) {
+  if (t == nullptr) {
+    set_error("%s: null table", op);
+    return RG_EINVAL;
+  }
+  if (t->n_chunks == 0) return RG_OK;
+  DeviceGuard guard(t->device);
+  const int tiles = (int)(kState8ChunkElems / kConvTileElems);
+  const dim3 grid((unsigned)(t->n_chunks * tiles)), block(kConvThreads);
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const bool nt = t->total_numel * 5 > ((int64_t)256 << 20);
+  if (write_codes) {
+    if (nt) hipLaunchKernelGGL((state8_kernel<true, true>), grid, block, 0, s, t->d_recs, tiles);
+    else hipLaunchKernelGGL((state8_kernel<true, false>), grid, block, 0, s, t->d_recs, tiles);
+  } else {
+    if (nt) hipLaunchKernelGGL((state8_kernel<false, true>), grid, block, 0, s, t->d_recs, tiles);
+    else hipLaunchKernelGGL((state8_kernel<false, false>), grid, block, 0, s, t->d_recs, tiles);
+  }
+  RG_HIP(hipGetLastError());
+  return RG_OK;
+}
+
+RG_API int rg_state8_quantize(rg_state8* t, void* stream) { return launch_state8(t, true, stream, "rg_state8_quantize"); }
+RG_API int rg_state8_dequantize(rg_state8* t, void* stream) { return launch_state8(t, false, stream, "rg_state8_dequantize"); }

@@ -16,7 +16,7 @@ from typing import Dict, List, Optional, Tuple
 import torch
 
 from . import _lib
-from .multi_tensor import dtype_code, stream_handle
+from .multi_tensor import State8Plan, allocate_state8, dtype_code, stream_handle
 
 try:        # the compiled module: lists of parameters walked in C++
     from . import _ranncgrad as _native
@@ -277,30 +277,36 @@ class _FusedBase(torch.optim.Optimizer):
             raise ValueError("gradient must be contiguous, on the parameter's device and of its size")
 
     def _table(self, key: Tuple, params: List[torch.Tensor], grads: List[torch.Tensor],
-               state1: Optional[List[torch.Tensor]], state2: Optional[List[torch.Tensor]]) -> _lib.OptimTable:
-        """Table for this exact list of parameters and gradient dtypes, re-pointed when any address moved."""
+               state1: Optional[List[torch.Tensor]], state2: Optional[List[torch.Tensor]],
+               scales: Optional[Tuple[List[torch.Tensor], List[torch.Tensor]]] = None) -> _lib.OptimTable:
+        """Table for this exact list of parameters and gradient dtypes, re-pointed when any address moved.  ``scales``:
+        the states are in 8 bits, and these are their blocks' scales."""
         copies = [self._model_copies.get(id(p)) for p in params]
         key = key + (tuple(g.dtype for g in grads),)
         ptrs = (tuple(p.data_ptr() for p in params), tuple(g.data_ptr() for g in grads),
                 tuple(s.data_ptr() for s in state1) if state1 is not None else None,
                 tuple(s.data_ptr() for s in state2) if state2 is not None else None,
                 tuple(c.data_ptr() if c is not None else 0 for c in copies))
+        scale_ptrs = tuple(tuple(s.data_ptr() for s in part) for part in scales) if scales is not None else (None, None)
+        ptrs += scale_ptrs
         hit = self._tables.get(key)
         dev = params[0].device
+        if hit is not None and scales is not None and hit[2][4] != (ptrs[2], ptrs[3]) + scale_ptrs:
+            hit = None          # 8-bit states have moved, which a table cannot follow: make another
         if hit is None:
             table = _lib.OptimTable(dev.index, ptrs[0], ptrs[1], ptrs[2], ptrs[3],
                                     ptrs[4] if any(ptrs[4]) else None, [p.numel() for p in params],
                                     [dtype_code(g.dtype) for g in grads],
-                                    [dtype_code(c.dtype) if c is not None else _lib.RG_F32 for c in copies])
+                                    [dtype_code(c.dtype) if c is not None else _lib.RG_F32 for c in copies], *scale_ptrs)
         else:
             table, old, _ = hit
             if old != ptrs:
-                table.update_pointers(ptrs[0], ptrs[1], ptrs[2], ptrs[3], ptrs[4] if any(ptrs[4]) else None,
-                                      stream_handle(dev))
+                state_ptrs = (ptrs[2], ptrs[3]) if scales is None else (None, None)
+                table.update_pointers(ptrs[0], ptrs[1], *state_ptrs, ptrs[4] if any(ptrs[4]) else None, stream_handle(dev))
         # the table borrows raw pointers: keep what it points at alive - except the gradients, which only have to
         # live until the launch that reads them is queued (their memory is reused in stream order) and whose
         # release lets the next backward find the same addresses free
-        self._tables[key] = (table, ptrs, [params, state1, state2, copies])
+        self._tables[key] = (table, ptrs, [params, state1, state2, copies, (ptrs[2], ptrs[3]) + scale_ptrs, scales])
         table.cache_key = key
         return table
 
@@ -311,8 +317,16 @@ class FusedAdam(_FusedBase):
     _decoupled = False
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, maximize=False,
-                 capturable=False):
-        """``capturable``: as in ``torch.optim.Adam`` - the step count lives on the device (``state["step"]`` is a
+                 capturable=False, state_bits=32):
+        """``state_bits=8``: both moments are held in 8 bits (``ranncgrad.h``, "optimizer states in 8 bits"): a byte an
+        element and a float32 scale for every 256 of them, a quarter of the memory and of the traffic.  The exp_avg_sq half is
+        held as its root, and a step rounds with a dither that depends on the step count and the element's place alone,
+        so that a run can be repeated bit for bit.  ``state[p]`` then has the codes under ``exp_avg`` / ``exp_avg_sq``
+        and the scales under ``exp_avg_scale`` / ``exp_avg_sq_scale``; ``state_dict()`` gives, and ``load_state_dict()``
+        takes, the float32 moments of ``torch.optim.Adam`` - converted on the GPU, which holds both forms meanwhile.  What
+        ``state_dict()`` gave loads back as the same codes and scales.  Everything else works as with 32 bits.
+
+        ``capturable``: as in ``torch.optim.Adam`` - the step count lives on the device (``state["step"]`` is a
         0-dim float32 GPU tensor), nothing about a step is decided on the host, and ``step()`` may be recorded in
         a HIP graph and replayed.  Every parameter of a group must then have a gradient at every step, at the same
         address (graph capture needs that anyway), and the first ``step()`` - which allocates the state - has to
@@ -326,13 +340,112 @@ class FusedAdam(_FusedBase):
         and, with ``grad_scale_ptr``, 1 / loss scale."""
         if lr < 0 or eps < 0 or not 0 <= betas[0] < 1 or not 0 <= betas[1] < 1 or weight_decay < 0:
             raise ValueError("invalid Adam hyper-parameters")
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits!r}")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, maximize=maximize))
         self.capturable = bool(capturable)
+        self.state_bits = int(state_bits)
         self._clocks: Dict[int, torch.Tensor] = {}       # group index -> its rg_adam_clock (8 float32 words on the device)
+        self._buffers8: Dict[int, List[Dict[str, torch.Tensor]]] = {}      # group index -> the buffers its 8-bit states lie in
+
+    def _make_moments(self, gi: int, params: List[torch.Tensor]) -> None:
+        """Zero moments for ``params`` of one group (``step`` is the caller's)."""
+        if self.state_bits == 32:
+            for p in params:
+                self.state[p]["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                self.state[p]["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+            return
+        if not params:
+            return
+        buffers: Dict[str, torch.Tensor] = {}
+        for name in ("exp_avg", "exp_avg_sq"):
+            codes, scales, buffers[name], buffers[name + "_scale"] = allocate_state8(params)
+            for p, c, s in zip(params, codes, scales):
+                self.state[p][name], self.state[p][name + "_scale"] = c, s
+        self._buffers8.setdefault(gi, []).append(buffers)
+
+    def _moments(self, params: List[torch.Tensor]):
+        """The state columns ``_table`` takes for these parameters."""
+        def column(name):
+            return [self.state[p][name] for p in params]
+        if self.state_bits == 32:
+            return column("exp_avg"), column("exp_avg_sq")
+        return column("exp_avg"), column("exp_avg_sq"), (column("exp_avg_scale"), column("exp_avg_sq_scale"))
+
+    def state_buffers(self, group: int = 0) -> Dict[str, torch.Tensor]:
+        """The flat buffers that hold a group's 8-bit states: ``exp_avg`` and ``exp_avg_sq`` (the codes, each parameter's at
+        a multiple of 256, in the group's order) and ``exp_avg_scale`` and ``exp_avg_sq_scale`` (a float for every 256)."""
+        if self.state_bits != 8:
+            raise RuntimeError("state_buffers: the states are in 32 bits, one tensor each")
+        held = self._buffers8.get(group, [])
+        if len(held) != 1:
+            raise RuntimeError("state_buffers: the group's states are not there yet" if not held else
+                               "state_buffers: the group's states came in more than one step and lie in several buffers")
+        return dict(held[0])
+
+    def _convert_moments(self, params: List[torch.Tensor], entries: List[Dict], to_codes: bool) -> None:
+        """Between the 8-bit states of ``params`` and the float32 moments in ``entries``."""
+        by_device: Dict[torch.device, List[int]] = {}
+        for i, p in enumerate(params):
+            by_device.setdefault(p.device, []).append(i)
+        for rows in by_device.values():
+            values, codes, scales, roots = [], [], [], []
+            for name in ("exp_avg", "exp_avg_sq"):
+                values += [entries[i][name] for i in rows]
+                codes += [self.state[params[i]][name] for i in rows]
+                scales += [self.state[params[i]][name + "_scale"] for i in rows]
+                roots += [name == "exp_avg_sq"] * len(rows)
+            plan = State8Plan(values, codes, scales, roots)
+            if to_codes:
+                plan.quantize()
+            else:
+                plan.dequantize()
+            plan.close()
+
+    def state_dict(self) -> Dict:
+        packed = super().state_dict()
+        if self.state_bits == 32:
+            return packed
+        # the packed entries are the live ones of ``self.state``: the float32 moments go into copies, and so does the step
+        # count, lest a later step made one of the two older than the other
+        params = [p for group in self.param_groups for p in group["params"]]
+        held = [(i, p) for i, p in enumerate(params) if "exp_avg_scale" in packed["state"].get(i, {})]
+        entries = []
+        for i, p in held:
+            entry = {k: v.clone() if torch.is_tensor(v) else v for k, v in packed["state"][i].items() if not k.startswith("exp_avg")}
+            entry["exp_avg"] = torch.empty(p.shape, dtype=torch.float32, device=p.device)
+            entry["exp_avg_sq"] = torch.empty(p.shape, dtype=torch.float32, device=p.device)
+            entries.append(entry)
+        self._convert_moments([p for _, p in held], entries, to_codes=False)
+        packed["state"] = dict(packed["state"])
+        packed["state"].update((i, entry) for (i, _), entry in zip(held, entries))
+        return packed
 
     def load_state_dict(self, state_dict) -> None:
         super().load_state_dict(state_dict)
         self._clocks.clear()          # re-seeded from the loaded ``step`` values by the next step
+        if self.state_bits == 32:
+            return
+        self._buffers8.clear()
+        for gi, group in enumerate(self.param_groups):
+            if all(p.is_cuda for p in group["params"]):       # otherwise they are converted by the step that needs them
+                self._settle_moments(gi, group["params"])
+
+    def _settle_moments(self, gi: int, params: List[torch.Tensor]) -> None:
+        """Loaded float32 moments among the states of ``params`` into 8 bits."""
+        if self.state_bits == 32:
+            return
+        loaded = [p for p in params if p.is_cuda and "exp_avg" in self.state.get(p, {}) and "exp_avg_scale" not in self.state[p]]
+        if not loaded:
+            return
+        entries = []
+        for p in loaded:
+            st = self.state[p]
+            if st["exp_avg"].numel() != p.numel() or st["exp_avg_sq"].numel() != p.numel():
+                raise ValueError("loaded moments differ in size from their parameter")
+            entries.append({k: st[k].to(p.device, torch.float32).contiguous() for k in ("exp_avg", "exp_avg_sq")})
+        self._make_moments(gi, loaded)
+        self._convert_moments(loaded, entries, to_codes=True)
 
     def _capturable_step(self, gi: int, group) -> None:
         """One group's step with its count on the device: advance the clock (one thread), then the update kernel."""
@@ -362,13 +475,10 @@ class FusedAdam(_FusedBase):
             counts = set()
             for p, g in zip(params, grads):
                 self._check_param(p, g)
-                st = self.state[p]
-                if len(st) == 0:
-                    st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-                    st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-                    counts.add(0)
-                else:
-                    counts.add(int(st["step"]))
+            fresh = [p for p in params if "exp_avg" not in self.state[p]]
+            counts.update(int(self.state[p]["step"]) if "exp_avg" in self.state[p] else 0 for p in params)
+            self._make_moments(gi, fresh)
+            self._settle_moments(gi, params)
             if len(counts) != 1:
                 raise RuntimeError("a capturable optimizer keeps one step count per group; the loaded counts differ")
             clock = torch.zeros(_lib.ADAM_CLOCK_BYTES // 4, dtype=torch.float32, device=dev)
@@ -379,9 +489,7 @@ class FusedAdam(_FusedBase):
             for p in params:
                 self.state[p]["step"] = clock[4]          # every parameter's count is the group's, on the device
             self._clocks[gi] = clock
-        ms = [self.state[p]["exp_avg"] for p in params]
-        vs = [self.state[p]["exp_avg_sq"] for p in params]
-        table = self._table((gi, "capturable"), params, grads, ms, vs)
+        table = self._table((gi, "capturable"), params, grads, *self._moments(params))
         b1, b2 = group["betas"]
         stream = stream_handle(dev)
         _lib.adam_clock_advance(clock.data_ptr(), group["lr"], b1, b2, self.gate, dev.index, stream)
@@ -415,6 +523,7 @@ class FusedAdam(_FusedBase):
             by_step: Dict[int, List[torch.Tensor]] = {}
             step_tensors = []
             grad_of: Dict[int, torch.Tensor] = {}
+            fresh = []
             for p in group["params"]:
                 g = self._grad_of(p)
                 if g is None:
@@ -422,10 +531,9 @@ class FusedAdam(_FusedBase):
                 self._check_param(p, g)
                 grad_of[id(p)] = g
                 st = self.state[p]
-                if len(st) == 0:
-                    st["step"] = torch.tensor(0.0, dtype=torch.float32)
-                    st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-                    st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                if "exp_avg" not in st:
+                    st.setdefault("step", torch.tensor(0.0, dtype=torch.float32))
+                    fresh.append(p)
                 # ``step`` stays a tensor (torch.optim's state layout); its integer value is mirrored
                 # here so that a step costs one batched increment instead of one tensor op per parameter
                 t = st["step"]
@@ -434,12 +542,12 @@ class FusedAdam(_FusedBase):
                 self._steps[id(p)] = (t, count)
                 step_tensors.append(t)
                 by_step.setdefault(count, []).append(p)
+            self._make_moments(gi, fresh)
+            self._settle_moments(gi, group["params"])
             if step_tensors:
                 torch._foreach_add_(step_tensors, 1)
             for step, ps in by_step.items():
-                ms = [self.state[p]["exp_avg"] for p in ps]
-                vs = [self.state[p]["exp_avg_sq"] for p in ps]
-                table = self._table((gi, tuple(id(p) for p in ps)), ps, [grad_of[id(p)] for p in ps], ms, vs)
+                table = self._table((gi, tuple(id(p) for p in ps)), ps, [grad_of[id(p)] for p in ps], *self._moments(ps))
                 b1, b2 = group["betas"]
                 self._scale_source(table).adam_step(group["lr"], b1, b2, group["eps"], group["weight_decay"], step,
                                 decoupled=self._decoupled, maximize=group["maximize"], grad_scale=self.grad_scale,
@@ -455,8 +563,8 @@ class FusedAdamW(FusedAdam):
     _decoupled = True
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, maximize=False,
-                 capturable=False):
-        super().__init__(params, lr, betas, eps, weight_decay, maximize, capturable)
+                 capturable=False, state_bits=32):
+        super().__init__(params, lr, betas, eps, weight_decay, maximize, capturable, state_bits)
 
 
 class FusedSGD(_FusedBase):

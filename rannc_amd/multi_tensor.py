@@ -6,7 +6,7 @@ runs in the HIP library.
 """
 from __future__ import annotations
 
-from typing import List, Optional, Sequence
+from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -203,6 +203,63 @@ class TensorPlan:
 
     def is_open(self) -> bool:
         return self.plan.is_open()
+
+
+class State8Plan:
+    """Optimizer states in 8 bits (``rg_state8`` in ``ranncgrad.h``) and the fp32 values they stand for, many tensors in one
+    launch: ``quantize()`` writes ``codes`` and ``scales`` from ``values``, ``dequantize()`` the other way round.
+
+    ``codes[i]`` is a float8_e4m3fn tensor of ``values[i]``'s size, ``scales[i]`` a float32 one with an element for every
+    256 of it (``allocate_state8`` makes both).  With ``root`` (one bool, or one per tensor) the values are second moments:
+    stored as their roots, read back as the roots' squares.  All tensors must be contiguous and on one GPU."""
+
+    def __init__(self, values: Sequence[torch.Tensor], codes: Sequence[torch.Tensor], scales: Sequence[torch.Tensor],
+                 root: Union[bool, Sequence[bool]] = False):
+        n = len(values)
+        roots = [bool(root)] * n if isinstance(root, (bool, int)) else [bool(r) for r in root]
+        if not n == len(codes) == len(scales) == len(roots):
+            raise ValueError("values, codes, scales and root differ in length")
+        self.device = values[0].device if n else torch.device("cuda", torch.cuda.current_device())
+        for i, (v, c, s) in enumerate(zip(values, codes, scales)):
+            for what, t, dtype, numel in (("values", v, torch.float32, v.numel()), ("codes", c, torch.float8_e4m3fn, v.numel()),
+                                          ("scales", s, torch.float32, _lib.state8_num_scales(v.numel()))):
+                _check_tensor(t, self.device, what, i)
+                if t.dtype != dtype:
+                    raise ValueError(f"{what}[{i}] is {t.dtype}, expected {dtype}")
+                if t.numel() != numel:
+                    raise ValueError(f"{what}[{i}] has {t.numel()} elements, expected {numel}")
+        self._keep = (list(values), list(codes), list(scales))        # the table points into these
+        self._table = _lib.State8Table(self.device.index, [c.data_ptr() for c in codes], [s.data_ptr() for s in scales],
+                                       [v.data_ptr() for v in values], [v.numel() for v in values], roots)
+
+    def quantize(self) -> None:
+        self._table.quantize(stream_handle(self.device))
+
+    def dequantize(self) -> None:
+        self._table.dequantize(stream_handle(self.device))
+
+    def close(self) -> None:
+        self._table.close()
+        self._keep = None
+
+    def is_open(self) -> bool:
+        return self._table.is_open()
+
+
+def allocate_state8(like: Sequence[torch.Tensor]) -> Tuple[List[torch.Tensor], List[torch.Tensor], torch.Tensor, torch.Tensor]:
+    """Zeroed 8-bit states for tensors on one GPU: ``(codes, scales, all codes, all scales)``.  The first two are views, of
+    the given tensors' shapes and one scale per block, into the flat last two, where each tensor starts at a whole block."""
+    numels = [t.numel() for t in like]
+    blocks = [_lib.state8_num_scales(n) for n in numels]
+    device = like[0].device
+    all_codes = torch.zeros(sum(blocks) * _lib.STATE8_BLOCK, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+    all_scales = torch.zeros(sum(blocks), dtype=torch.float32, device=device)
+    codes, scales, at = [], [], 0
+    for t, n, b in zip(like, numels, blocks):
+        codes.append(all_codes[at * _lib.STATE8_BLOCK:at * _lib.STATE8_BLOCK + n].view(t.shape))
+        scales.append(all_scales[at:at + b])
+        at += b
+    return codes, scales, all_codes, all_scales
 
 
 def fill_zero_(t: torch.Tensor) -> torch.Tensor:
