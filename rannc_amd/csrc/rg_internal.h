@@ -186,6 +186,7 @@ hipError_t launch_fill_zero(void* dst, int64_t nbytes, hipStream_t stream);
 
 constexpr int64_t kMaxTensorElems = (int64_t)1 << 44;   // 16 TiB of codes: keeps the sums of sizes far from overflow
 constexpr int kState8Block = RG_STATE8_BLOCK;   // elements that share a scale
+constexpr int64_t kOpt8ChunkElems = 8192;       // elements of a full chunk record below
 
 // One row of the work table of an optimizer step with 8-bit states: a run of whole blocks of one parameter (the last
 // block may be shorter).
@@ -221,11 +222,10 @@ struct Adam8Args {
   const float* grad_scale_dev;  // optional: the gradient scale lives on the device
   float grad_scale_sign;        // ... and is multiplied by this (-1: maximize)
   uint32_t step;
-  int32_t tiles_per_chunk;
   Adam8Const c;
 };
 
-hipError_t launch_adam8(const Adam8Args& a, int64_t n_chunks, int64_t chunk_elems, bool streaming, hipStream_t stream);
+hipError_t launch_adam8(const Adam8Args& a, int64_t n_chunks, bool streaming, hipStream_t stream);
 // Ticks of the current device's wall clock that a wavefront of a large flat fill waits before it stores (0: unknown rate).
 int fill_delay_ticks();
 int fill_delay_ticks(int ns);   // the same clock, another delay

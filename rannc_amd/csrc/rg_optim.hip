@@ -433,6 +433,7 @@ static int create_table(rg_optim** out, int device, int n, const OptColumns& a, 
   o->device = device;
   o->n_tensors = n;
   o->state8 = state8;
+  if (state8) o->chunk_elems = kOpt8ChunkElems;
   o->has_state1 = state8 || a.state1 != nullptr;
   o->has_state2 = state8 || a.state2 != nullptr;
   o->rows.resize((size_t)n);
@@ -630,7 +631,7 @@ static int adam_step(rg_optim* o, const rg_adam_args* g, const rg_adam_clock* cl
     a.c.inv_bias2_sqrt = 1.0f / (float)sqrt(bias2);
     a.c.eps = (float)g->eps;
     DeviceGuard guard(o->device);
-    RG_HIP(launch_adam8(a, o->n_chunks, o->chunk_elems, o->total_numel * 18 > ((int64_t)256 << 20),
+    RG_HIP(launch_adam8(a, o->n_chunks, o->total_numel * 18 > ((int64_t)256 << 20),
                         reinterpret_cast<hipStream_t>(stream)));
     return RG_OK;
   }

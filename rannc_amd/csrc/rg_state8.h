@@ -42,6 +42,22 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
   return ab > cd ? ab : cd;
 }
 
+// Of two numbers per lane at once: lanes 0-31 get the largest `a`, lanes 32-63 the largest `b`.  The halves trade places
+// (a's upper for b's lower), then the two rows of each half, then the rotations above.
+__device__ __forceinline__ uint32_t half_max(uint32_t a, uint32_t b) {
+  const u32x2 halves = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(a, b, false, false));
+  uint32_t x = halves.x > halves.y ? halves.x : halves.y;
+  const u32x2 rows = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(x, x, false, false));
+  x = rows.x > rows.y ? rows.x : rows.y;
+  x = max_row_ror<1>(x);
+  x = max_row_ror<2>(x);
+  x = max_row_ror<4>(x);
+  return max_row_ror<8>(x);
+}
+__device__ __forceinline__ float read_lane_f32(float x, int lane) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), lane));
+}
+
 // What a block stores as its scale, and the factor to e4m3's range; inv == 0: every code of the block is zero.
 struct BlockScale {
   float s, inv;

@@ -14,7 +14,7 @@ namespace rg {
 namespace {
 
 constexpr int kLaneElems = 4;                                   // elements of a block one lane holds: 64 lanes, 256 elements
-constexpr int kAdam8Threads = 256, kAdam8TileElems = 4096;      // 4 wavefronts, 4 blocks each
+constexpr int kAdam8Threads = 128, kAdam8TileElems = 512;       // 2 wavefronts, a block each
 constexpr int kConvThreads = 256, kConvTileElems = 4096;
 
 template <int DT> __device__ __forceinline__ float load_one(const char* p) { return __uint_as_float(load_u32(p)); }
@@ -59,63 +59,155 @@ template <bool NT> __device__ __forceinline__ void store_codes4(char* p, int n, 
     if (j < n) store_u8(p + j, (w >> (8 * j)) & 0xffu);
 }
 
-// One block of 256 elements (fewer at a tensor's end) by one wavefront.
-template <int G, int C, bool NT>
+// Hand-out order of a launch's tiles: workgroups are dealt to the eight XCDs in turn, and runs of kXcdRun consecutive
+// tiles go to one of them (an incomplete last round keeps its order).
+constexpr unsigned kXcdRun = 64;
+__device__ __forceinline__ unsigned tile_of_block() {
+  const unsigned b = blockIdx.x, round = b / (8u * kXcdRun) * (8u * kXcdRun);
+  if (round + 8u * kXcdRun > gridDim.x) return b;
+  const unsigned in = b - round;
+  return round + (in % 8u) * kXcdRun + in / 8u;
+}
+
+// Stores of a wavefront's lanes side by side at `base` (the same for all lanes): streaming ones as raw buffer stores with
+// the policy "sc1 nt".
+constexpr int kStreamAux = 18;
+template <bool NT> __device__ __forceinline__ void put16(char* base, uint32_t off, u32x4 v) {
+  if (NT) __builtin_amdgcn_raw_buffer_store_b128(v, __builtin_amdgcn_make_buffer_rsrc(base, 0, -1, 0x00020000), off, 0, kStreamAux);
+  else st16<false>(base + off, v);
+}
+template <bool NT> __device__ __forceinline__ void put8(char* base, uint32_t off, u32x2 v) {
+  if (NT) __builtin_amdgcn_raw_buffer_store_b64(v, __builtin_amdgcn_make_buffer_rsrc(base, 0, -1, 0x00020000), off, 0, kStreamAux);
+  else st8<false>(base + off, v);
+}
+template <bool NT> __device__ __forceinline__ void put4(char* base, uint32_t off, uint32_t v) {
+  if (NT) __builtin_amdgcn_raw_buffer_store_b32(v, __builtin_amdgcn_make_buffer_rsrc(base, 0, -1, 0x00020000), off, 0, kStreamAux);
+  else st_codes<false>(base + off, v);
+}
+template <int DT, bool NT> __device__ __forceinline__ void put_raw(char* base, int lane, const Raw<DT, 4>& r) {
+  if constexpr (DT == RG_F32) put16<NT>(base, (uint32_t)lane * 16u, r.v);
+  else put8<NT>(base, (uint32_t)lane * 8u, r.v);
+}
+
+__device__ __forceinline__ float maximum_abs3(float a, float b, float c) {   // NaN if any is
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(__builtin_fabsf(a), __builtin_fabsf(b)), __builtin_fabsf(c));
+}
+
+// Square root, correctly rounded, for 2^-100 <= x < infinity; NaN for anything smaller than 2^-126 (zero too) and for
+// infinity.  The estimate x * rsq(x) is off by at most a few units; its residual x - s^2 is exact in one fma, and s +
+// residual / (2 s) then rounds as the root itself does: checked for every fp32 number of the range.
+__device__ __forceinline__ float sqrt_normal(float x) {
+  const float y = __builtin_amdgcn_rsqf(x);
+  const float s = x * y;
+  return __builtin_fmaf(__builtin_fmaf(-s, s, x), 0.5f * y, s);
+}
+
+constexpr float kRootShift = 16777216.0f;                       // 2^24: the step's roots are carried times this, squares times 2^48
+constexpr float kSquareShift = 281474976710656.0f;
+
+// One block of 256 elements (fewer at a tensor's end) by one wavefront, four per lane.
+template <int G, int C, bool NT, bool FULL>
 __device__ __forceinline__ void adam8_block(const Opt8ChunkRec& r, int start, int lane, const Adam8Const& c, float coef,
                                             uint32_t step) {
-  const int e = start + lane * kLaneElems;
-  const int n = r.len - e;                 // <= 0: this lane has no element
   constexpr int CD = C >= 0 ? C : RG_F32;
-  char* pp = reinterpret_cast<char*>(r.param) + (ptrdiff_t)e * 4;
-  const char* gp = reinterpret_cast<const char*>(r.grad) + (ptrdiff_t)e * ElemSize<G>::value;
-  char* c1 = reinterpret_cast<char*>(r.codes1) + e;
-  char* c2 = reinterpret_cast<char*>(r.codes2) + e;
+  constexpr int GS = ElemSize<G>::value, CS = ElemSize<CD>::value;
   const int block = start / kState8Block;
-  float p[4], g[4], m[4], v[4];
-  load4<RG_F32, NT>(pp, n, p);
-  load4<G, NT>(gp, n, g);
-  const uint32_t w1 = load_codes4<NT>(c1, n), w2 = load_codes4<NT>(c2, n);
-  const float k1 = __uint_as_float(load_u32(reinterpret_cast<const char*>(r.scales1 + block))) * 0.00390625f;
-  const float k2 = __uint_as_float(load_u32(reinterpret_cast<const char*>(r.scales2 + block))) * 0.00390625f;
-  decode(w1, k1, m);
-  decode(w2, k2, v);
+  const int n = FULL ? kLaneElems : r.len - start - lane * kLaneElems;       // <= 0: this lane has no element
+  char* pp = reinterpret_cast<char*>(r.param) + (size_t)start * 4;
+  const char* gp = reinterpret_cast<const char*>(r.grad) + (size_t)start * GS;
+  char* c1 = reinterpret_cast<char*>(r.codes1) + start;
+  char* c2 = reinterpret_cast<char*>(r.codes2) + start;
+  char* cp = reinterpret_cast<char*>(r.copy) + (size_t)start * CS;
+  float p[4], g[4], m[4], q[4];
+  load4<RG_F32, NT>(pp + lane * 16, n, p);
+  load4<G, NT>(gp + lane * (4 * GS), n, g);
+  const uint32_t w1 = load_codes4<NT>(c1 + lane * 4, n), w2 = load_codes4<NT>(c2 + lane * 4, n);
+  const float s1_old = r.scales1[block], s2_old = r.scales2[block];
+  decode(w1, s1_old * 0.00390625f, m);                                       // s / 256
+  decode(w2, s2_old * (0.00390625f * kRootShift), q);
+  if (c.grad_scale != 1.0f) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[j] = g[j] * c.grad_scale;
+  }
+  if (coef != 1.0f) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[j] = g[j] * coef;
+  }
+  if (c.param_mul != 1.0f) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p[j] = p[j] * c.param_mul;
+  }
+  if (c.weight_decay != 0.0f) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[j] = g[j] + c.weight_decay * p[j];
+  }
   float root[4];
-  uint32_t top1 = 0, top2 = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    float gj = g[j] * c.grad_scale;
-    gj = gj * coef;
-    p[j] = p[j] * c.param_mul;
-    if (c.weight_decay != 0.0f) gj = gj + c.weight_decay * p[j];
-    m[j] = c.beta1 * m[j] + c.one_minus_beta1 * gj;
-    const float vj = c.beta2 * (v[j] * v[j]) + (c.one_minus_beta2 * gj) * gj;
-    root[j] = sqrtf(vj);
-    p[j] = p[j] + (c.neg_step_size * m[j]) / (root[j] * c.inv_bias2_sqrt + c.eps);
-    const uint32_t a = magnitude_bits(m[j]), b = magnitude_bits(root[j]);
-    top1 = top1 > a ? top1 : a;
-    top2 = top2 > b ? top2 : b;
+    m[j] = c.beta1 * m[j] + c.one_minus_beta1 * g[j];
+    root[j] = sqrt_normal(c.beta2 * (q[j] * q[j]) + (c.one_minus_beta2 * kSquareShift * g[j]) * g[j]);
   }
-  const BlockScale s1 = block_scale(wave_max(top1)), s2 = block_scale(wave_max(top2));
-  const uint32_t place = (r.first + (uint32_t)e) * kDitherPlace;
+  float top2 = __builtin_elementwise_maximum(maximum_abs3(root[0], root[1], root[2]), root[3]);
+  const bool plain = __builtin_amdgcn_ballot_w64(top2 != top2) == 0;
+  if (!plain) {      // some second moment is zero, subnormal or not a number: the roots one by one
+    top2 = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float old = q[j] * (1.0f / kRootShift);
+      root[j] = sqrtf(c.beta2 * (old * old) + (c.one_minus_beta2 * g[j]) * g[j]) * kRootShift;
+      top2 = __builtin_elementwise_maximum(top2, __builtin_fabsf(root[j]));
+    }
+  }
+  const float top1 = __builtin_elementwise_maximum(maximum_abs3(m[0], m[1], m[2]), __builtin_fabsf(m[3]));
+  const float inv_bias = c.inv_bias2_sqrt * (1.0f / kRootShift);
+  if (plain) {       // the denominators are normal numbers: a reciprocal (1 unit) in place of the division
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p[j] = p[j] + (c.neg_step_size * m[j]) * __builtin_amdgcn_rcpf(root[j] * inv_bias + c.eps);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p[j] = p[j] + (c.neg_step_size * m[j]) / (root[j] * inv_bias + c.eps);
+  }
+  if (FULL) put_raw<RG_F32, NT>(pp, lane, Codec<RG_F32, 4>::pack(p));
+  else store4<RG_F32, NT>(pp + lane * 16, n, p);
+  if constexpr (C >= 0) {
+    if (FULL) put_raw<CD, NT>(cp, lane, Codec<CD, 4>::pack(p));
+    else store4<CD, NT>(cp + lane * (4 * CS), n, p);
+  }
+
+  // Both moments' largest at once: the lower half of the wavefront ends up with the first's, the upper with the root's.
+  const uint32_t top = half_max(magnitude_bits(top1), magnitude_bits(top2));
+  const float shift = lane < 32 ? 1.0f : 1.0f / kRootShift;
+  const float s = __uint_as_float(top) * shift;
+  const bool number = top < 0x7f800000u, holds = number && s >= __uint_as_float(kState8TinyBits);
+  const float inv = holds ? 256.0f * (1.0f / __uint_as_float(top)) : 0.0f;
+  const float kept = holds ? s : number ? 0.0f : __uint_as_float(0x7fc00000u);
+  const float inv1 = read_lane_f32(inv, 0), inv2 = read_lane_f32(inv, 32);
+  if ((lane & 31) == 0) store1<RG_F32>(reinterpret_cast<char*>((lane == 0 ? r.scales1 : r.scales2) + block), kept);
+
+  const uint32_t place = (r.first + (uint32_t)start) * kDitherPlace, u = (uint32_t)lane * (kLaneElems * kDitherPlace);
   uint32_t o1 = 0, o2 = 0;
-  float y[4];
-  if (s1.inv != 0.0f) {
+  if (inv1 != 0.0f) {
+    float y[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = to_range<false>(m[j], s1.inv);
-    o1 = encode_dithered(y, place + step * kDitherFirst);
+    for (int j = 0; j < 4; ++j) y[j] = m[j] * inv1;
+    o1 = encode_dithered(y, u + (place + step * kDitherFirst));
   }
-  if (s2.inv != 0.0f) {
+  if (inv2 != 0.0f) {
+    float y[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = to_range<true>(root[j], s2.inv);
-    o2 = encode_dithered(y, place + step * kDitherRoot);
+    for (int j = 0; j < 4; ++j) y[j] = fmaxf(root[j] * inv2, kState8MinRoot);
+    if (!plain) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = root[j] > 0.0f ? y[j] : 0.0f;
+    }
+    o2 = encode_dithered(y, u + (place + step * kDitherRoot));
   }
-  store4<RG_F32, NT>(pp, n, p);
-  if (C >= 0) store4<CD, NT>(reinterpret_cast<char*>(r.copy) + (ptrdiff_t)e * ElemSize<CD>::value, n, p);
-  store_codes4<NT>(c1, n, o1);
-  store_codes4<NT>(c2, n, o2);
-  if (lane == 0) {
-    store_u32(reinterpret_cast<char*>(r.scales1 + block), __float_as_uint(s1.s));
-    store_u32(reinterpret_cast<char*>(r.scales2 + block), __float_as_uint(s2.s));
+  if (FULL) {
+    put4<NT>(c1, (uint32_t)lane * 4u, o1);
+    put4<NT>(c2, (uint32_t)lane * 4u, o2);
+  } else {
+    store_codes4<NT>(c1 + lane * 4, n, o1);
+    store_codes4<NT>(c2 + lane * 4, n, o2);
   }
 }
 
@@ -133,17 +225,19 @@ __global__ __launch_bounds__(kAdam8Threads) void adam8_kernel(Adam8Args a) {
     a.c.neg_step_size = a.clock->neg_step_size;
     a.c.inv_bias2_sqrt = 1.0f / a.clock->bias2_sqrt;
   }
-  const unsigned bid = blockIdx.x;
-  const Opt8ChunkRec r = a.chunks[bid / (unsigned)a.tiles_per_chunk];
+  constexpr unsigned kTiles = (unsigned)(kOpt8ChunkElems / kAdam8TileElems);
+  const unsigned t = tile_of_block();
+  const Opt8ChunkRec r = a.chunks[t / kTiles];
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64u)), lane = (int)(threadIdx.x % 64u);
-  constexpr int kWaveElems = kAdam8TileElems / (kAdam8Threads / 64);
-  const int start = (int)(bid % (unsigned)a.tiles_per_chunk) * kAdam8TileElems + wave * kWaveElems;
+  const int start = (int)(t % kTiles) * kAdam8TileElems + wave * kState8Block;
+  if (start >= r.len) return;
+  const bool full = r.len - start >= kState8Block;
   const int copy_kind = r.copy ? r.copy_dtype : -1;
-#define RG_ADAM8(G, C)                                                                                  \
-  if (r.grad_dtype == G && copy_kind == C) {                                                            \
-    for (int b = start; b < start + kWaveElems && b < r.len; b += kState8Block)                         \
-      adam8_block<G, C, NT>(r, b, lane, a.c, coef, step);                                               \
-    return;                                                                                             \
+#define RG_ADAM8(G, C)                                                    \
+  if (r.grad_dtype == G && copy_kind == C) {                              \
+    if (full) adam8_block<G, C, NT, true>(r, start, lane, a.c, coef, step); \
+    else adam8_block<G, C, NT, false>(r, start, lane, a.c, coef, step);   \
+    return;                                                               \
   }
   RG_ADAM8(RG_F32, -1)
   RG_ADAM8(RG_F32, RG_BF16)
@@ -229,10 +323,8 @@ __global__ __launch_bounds__(kConvThreads) void state8_kernel(const State8Rec* r
 
 }  // namespace
 
-hipError_t launch_adam8(const Adam8Args& args, int64_t n_chunks, int64_t chunk_elems, bool streaming, hipStream_t stream) {
-  Adam8Args a = args;
-  a.tiles_per_chunk = (int32_t)((chunk_elems + kAdam8TileElems - 1) / kAdam8TileElems);
-  const dim3 grid((unsigned)(n_chunks * a.tiles_per_chunk)), block(kAdam8Threads);
+hipError_t launch_adam8(const Adam8Args& a, int64_t n_chunks, bool streaming, hipStream_t stream) {
+  const dim3 grid((unsigned)(n_chunks * (kOpt8ChunkElems / kAdam8TileElems))), block(kAdam8Threads);
   if (streaming) hipLaunchKernelGGL((adam8_kernel<true>), grid, block, 0, stream, a);
   else hipLaunchKernelGGL((adam8_kernel<false>), grid, block, 0, stream, a);
   return hipGetLastError();
