@@ -24,26 +24,14 @@ constexpr uint32_t kDitherPlace = 0xD1B54A33u, kDitherFirst = 0xABC98389u, kDith
 
 __device__ __forceinline__ uint32_t magnitude_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// Largest of one unsigned number per lane, the same for all (all 64 lanes active): a rotation within the rows of 16
-// lanes leaves every lane its row's largest, the four rows meet in scalar registers.  On magnitudes' bits the order is
-// that of the numbers with infinity above them and NaN above that, so a NaN is not lost on the way.
+// The largest of two numbers per lane, both at once: lanes 0-31 get the largest `a`, lanes 32-63 the largest `b` (all 64
+// lanes active).  The halves trade places (a's upper for b's lower), then the two rows of 16 lanes of each half, then
+// rotations within a row: 8 instructions, where two reductions of 64 lanes one after the other take 22.  On magnitudes'
+// bits the order is that of the numbers with infinity above them and NaN above that, so neither is lost on the way.
 template <int N> __device__ __forceinline__ uint32_t max_row_ror(uint32_t x) {
   const uint32_t y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x120 + N, 0xf, 0xf, true);
   return x > y ? x : y;
 }
-__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-  x = max_row_ror<1>(x);
-  x = max_row_ror<2>(x);
-  x = max_row_ror<4>(x);
-  x = max_row_ror<8>(x);
-  const uint32_t a = (uint32_t)__builtin_amdgcn_readlane((int)x, 0), b = (uint32_t)__builtin_amdgcn_readlane((int)x, 16);
-  const uint32_t c = (uint32_t)__builtin_amdgcn_readlane((int)x, 32), d = (uint32_t)__builtin_amdgcn_readlane((int)x, 48);
-  const uint32_t ab = a > b ? a : b, cd = c > d ? c : d;
-  return ab > cd ? ab : cd;
-}
-
-// Of two numbers per lane at once: lanes 0-31 get the largest `a`, lanes 32-63 the largest `b`.  The halves trade places
-// (a's upper for b's lower), then the two rows of each half, then the rotations above.
 __device__ __forceinline__ uint32_t half_max(uint32_t a, uint32_t b) {
   const u32x2 halves = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(a, b, false, false));
   uint32_t x = halves.x > halves.y ? halves.x : halves.y;
@@ -58,22 +46,18 @@ __device__ __forceinline__ float read_lane_f32(float x, int lane) {
   return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), lane));
 }
 
-// What a block stores as its scale, and the factor to e4m3's range; inv == 0: every code of the block is zero.
+// What a block stores as its scale, and the factor that takes its elements to e4m3's range (inv == 0: every code of the
+// block is zero).  `max_bits` may belong to elements that are carried times 1 / shift, a power of two.
 struct BlockScale {
   float s, inv;
 };
-__device__ __forceinline__ BlockScale block_scale(uint32_t max_bits) {
-  if (max_bits >= 0x7f800000u) return {__uint_as_float(0x7fc00000u), 0.0f};
-  if (max_bits < kState8TinyBits) return {0.0f, 0.0f};
-  const float s = __uint_as_float(max_bits);
-  return {s, 256.0f * (1.0f / s)};      // 1 / s correctly rounded; s * inv rounds to 256 at most
-}
-
-// x in units of the block's e4m3 range.  A root that is not zero does not become zero: the step divides by it.
-template <bool ROOT> __device__ __forceinline__ float to_range(float x, float inv) {
-  const float y = x * inv;
-  if (ROOT) return y > 0.0f ? fmaxf(y, kState8MinRoot) : y;
-  return y;
+__device__ __forceinline__ BlockScale block_scale(uint32_t max_bits, float shift) {
+  const float top = __uint_as_float(max_bits), s = top * shift;
+  const bool number = max_bits < 0x7f800000u, holds = number && s >= __uint_as_float(kState8TinyBits);
+  BlockScale out;
+  out.s = holds ? s : number ? 0.0f : __uint_as_float(0x7fc00000u);
+  out.inv = holds ? 256.0f * (1.0f / top) : 0.0f;       // 1 / top correctly rounded: top * inv rounds to 256 at most
+  return out;
 }
 
 // Four elements of a block to their codes, to nearest (ties to even) or dithered by four numbers of 32 bits, of which the

@@ -15,7 +15,8 @@ namespace {
 
 constexpr int kLaneElems = 4;                                   // elements of a block one lane holds: 64 lanes, 256 elements
 constexpr int kAdam8Threads = 128, kAdam8TileElems = 512;       // 2 wavefronts, a block each
-constexpr int kConvThreads = 256, kConvTileElems = 4096;
+constexpr int kConvThreads = 128, kConvTileElems = 1024;        // 2 wavefronts, two blocks each
+constexpr int64_t kState8ChunkElems = 8192;                     // elements of a full record of a conversion's table
 
 template <int DT> __device__ __forceinline__ float load_one(const char* p) { return __uint_as_float(load_u32(p)); }
 template <> __device__ __forceinline__ float load_one<RG_F16>(const char* p) {
@@ -61,12 +62,13 @@ template <bool NT> __device__ __forceinline__ void store_codes4(char* p, int n, 
 
 // Hand-out order of a launch's tiles: workgroups are dealt to the eight XCDs in turn, and runs of kXcdRun consecutive
 // tiles go to one of them (an incomplete last round keeps its order).
-constexpr unsigned kXcdRun = 64;
-__device__ __forceinline__ unsigned tile_of_block() {
-  const unsigned b = blockIdx.x, round = b / (8u * kXcdRun) * (8u * kXcdRun);
-  if (round + 8u * kXcdRun > gridDim.x) return b;
+constexpr unsigned kXcdRun = 224;
+constexpr unsigned kConvXcdRun = 64;
+template <unsigned RUN> __device__ __forceinline__ unsigned tile_of_block() {
+  const unsigned b = blockIdx.x, round = b / (8u * RUN) * (8u * RUN);
+  if (round + 8u * RUN > gridDim.x) return b;
   const unsigned in = b - round;
-  return round + (in % 8u) * kXcdRun + in / 8u;
+  return round + (in % 8u) * RUN + in / 8u;
 }
 
 // Stores of a wavefront's lanes side by side at `base` (the same for all lanes): streaming ones as raw buffer stores with
@@ -175,14 +177,9 @@ __device__ __forceinline__ void adam8_block(const Opt8ChunkRec& r, int start, in
   }
 
   // Both moments' largest at once: the lower half of the wavefront ends up with the first's, the upper with the root's.
-  const uint32_t top = half_max(magnitude_bits(top1), magnitude_bits(top2));
-  const float shift = lane < 32 ? 1.0f : 1.0f / kRootShift;
-  const float s = __uint_as_float(top) * shift;
-  const bool number = top < 0x7f800000u, holds = number && s >= __uint_as_float(kState8TinyBits);
-  const float inv = holds ? 256.0f * (1.0f / __uint_as_float(top)) : 0.0f;
-  const float kept = holds ? s : number ? 0.0f : __uint_as_float(0x7fc00000u);
-  const float inv1 = read_lane_f32(inv, 0), inv2 = read_lane_f32(inv, 32);
-  if ((lane & 31) == 0) store1<RG_F32>(reinterpret_cast<char*>((lane == 0 ? r.scales1 : r.scales2) + block), kept);
+  const BlockScale s = block_scale(half_max(magnitude_bits(top1), magnitude_bits(top2)), lane < 32 ? 1.0f : 1.0f / kRootShift);
+  const float inv1 = read_lane_f32(s.inv, 0), inv2 = read_lane_f32(s.inv, 32);
+  if ((lane & 31) == 0) store1<RG_F32>(reinterpret_cast<char*>((lane == 0 ? r.scales1 : r.scales2) + block), s.s);
 
   const uint32_t place = (r.first + (uint32_t)start) * kDitherPlace, u = (uint32_t)lane * (kLaneElems * kDitherPlace);
   uint32_t o1 = 0, o2 = 0;
@@ -226,7 +223,7 @@ __global__ __launch_bounds__(kAdam8Threads) void adam8_kernel(Adam8Args a) {
     a.c.inv_bias2_sqrt = 1.0f / a.clock->bias2_sqrt;
   }
   constexpr unsigned kTiles = (unsigned)(kOpt8ChunkElems / kAdam8TileElems);
-  const unsigned t = tile_of_block();
+  const unsigned t = tile_of_block<kXcdRun>();
   const Opt8ChunkRec r = a.chunks[t / kTiles];
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64u)), lane = (int)(threadIdx.x % 64u);
   const int start = (int)(t % kTiles) * kAdam8TileElems + wave * kState8Block;
@@ -266,59 +263,116 @@ struct State8Rec {
 };
 static_assert(sizeof(State8Rec) == 32, "conversion record must stay 32 bytes");
 
-template <bool ROOT, bool NT>
-__device__ __forceinline__ void quantize_block(const State8Rec& r, int start, int lane) {
-  const int e = start + lane * kLaneElems;
-  const int n = r.len - e;
-  float x[4];
-  load4<RG_F32, NT>(reinterpret_cast<const char*>(r.values) + (ptrdiff_t)e * 4, n, x);
-  uint32_t top = 0;
+// The magnitudes to be stored: the values, or their roots (times 2^24).  `plain`: no root is zero or not a number.
+template <bool ROOT> __device__ __forceinline__ bool stored_form(float (&x)[4], float& top) {
+  if (!ROOT) {
+    top = __builtin_elementwise_maximum(maximum_abs3(x[0], x[1], x[2]), __builtin_fabsf(x[3]));
+    return true;
+  }
+  float r[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r[j] = sqrt_normal(x[j] * kSquareShift);
+  top = __builtin_elementwise_maximum(maximum_abs3(r[0], r[1], r[2]), r[3]);
+  const bool plain = __builtin_amdgcn_ballot_w64(top != top) == 0;
+  if (!plain) {
+    top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      r[j] = sqrtf(x[j]) * kRootShift;
+      top = __builtin_elementwise_maximum(top, __builtin_fabsf(r[j]));
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] = r[j];
+  return plain;
+}
+template <bool ROOT> __device__ __forceinline__ uint32_t nearest_codes(const float (&x)[4], float inv, bool plain) {
+  if (inv == 0.0f) return 0;
+  float y[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    if (ROOT) x[j] = sqrtf(x[j]);
-    const uint32_t a = magnitude_bits(x[j]);
-    top = top > a ? top : a;
+    y[j] = x[j] * inv;
+    if (ROOT) {
+      y[j] = fmaxf(y[j], kState8MinRoot);
+      if (!plain) y[j] = x[j] > 0.0f ? y[j] : 0.0f;
+    }
   }
-  const BlockScale s = block_scale(wave_max(top));
-  uint32_t w = 0;
-  if (s.inv != 0.0f) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = to_range<ROOT>(x[j], s.inv);
-    w = encode_nearest(x);
-  }
-  store_codes4<NT>(reinterpret_cast<char*>(r.codes) + e, n, w);
-  if (lane == 0) store_u32(reinterpret_cast<char*>(r.scales + start / kState8Block), __float_as_uint(s.s));
+  return encode_nearest(y);
 }
 
-template <bool ROOT, bool NT>
-__device__ __forceinline__ void dequantize_block(const State8Rec& r, int start, int lane) {
-  const int e = start + lane * kLaneElems;
-  const int n = r.len - e;
-  const float k = __uint_as_float(load_u32(reinterpret_cast<const char*>(r.scales + start / kState8Block))) * 0.00390625f;
-  float x[4];
-  decode(load_codes4<NT>(reinterpret_cast<const char*>(r.codes) + e, n), k, x);
+// Two consecutive blocks by one wavefront (the second may be missing, either may end early), so that one reduction
+// finds both largest magnitudes.
+template <bool ROOT, bool NT, bool FULL>
+__device__ __forceinline__ void quantize_pair(const State8Rec& r, int start, int lane) {
+  const char* vp = reinterpret_cast<const char*>(r.values) + (size_t)start * 4;
+  char* cp = reinterpret_cast<char*>(r.codes) + start;
+  const int na = FULL ? kLaneElems : r.len - start - lane * kLaneElems, nb = FULL ? kLaneElems : na - kState8Block;
+  float a[4], b[4], top_a, top_b;
+  load4<RG_F32, NT>(vp + lane * 16, na, a);
+  load4<RG_F32, NT>(vp + (kState8Block * 4 + lane * 16), nb, b);
+  const bool plain_a = stored_form<ROOT>(a, top_a), plain_b = stored_form<ROOT>(b, top_b);
+  const BlockScale s = block_scale(half_max(magnitude_bits(top_a), magnitude_bits(top_b)), ROOT ? 1.0f / kRootShift : 1.0f);
+  const uint32_t wa = nearest_codes<ROOT>(a, read_lane_f32(s.inv, 0), plain_a);
+  const uint32_t wb = nearest_codes<ROOT>(b, read_lane_f32(s.inv, 32), plain_b);
+  if (FULL) {
+    put4<NT>(cp, (uint32_t)lane * 4u, wa);
+    put4<NT>(cp, (uint32_t)lane * 4u + kState8Block, wb);
+  } else {
+    store_codes4<NT>(cp + lane * 4, na, wa);
+    store_codes4<NT>(cp + (kState8Block + lane * 4), nb, wb);
+  }
+  const int block = start / kState8Block + (lane >> 5);
+  if ((lane & 31) == 0 && block * kState8Block < r.len) store1<RG_F32>(reinterpret_cast<char*>(r.scales + block), s.s);
+}
+
+template <bool ROOT, bool NT, bool FULL>
+__device__ __forceinline__ void dequantize_pair(const State8Rec& r, int start, int lane) {
+  char* vp = reinterpret_cast<char*>(r.values) + (size_t)start * 4;
+  const char* cp = reinterpret_cast<const char*>(r.codes) + start;
+  const int na = FULL ? kLaneElems : r.len - start - lane * kLaneElems, nb = FULL ? kLaneElems : na - kState8Block;
+  const uint32_t wa = load_codes4<NT>(cp + lane * 4, na), wb = load_codes4<NT>(cp + (kState8Block + lane * 4), nb);
+  const int block = start / kState8Block;
+  const bool second = FULL || r.len - start > kState8Block;
+  const float sa = r.scales[block], sb = second ? r.scales[block + 1] : 0.0f;
+  float a[4], b[4];
+  decode(wa, sa * 0.00390625f, a);
+  decode(wb, sb * 0.00390625f, b);
   if (ROOT) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = x[j] * x[j];
+    for (int j = 0; j < 4; ++j) {
+      a[j] = a[j] * a[j];
+      b[j] = b[j] * b[j];
+    }
   }
-  store4<RG_F32, NT>(reinterpret_cast<char*>(r.values) + (ptrdiff_t)e * 4, n, x);
+  if (FULL) {
+    put16<NT>(vp, (uint32_t)lane * 16u, Codec<RG_F32, 4>::pack(a).v);
+    put16<NT>(vp, (uint32_t)lane * 16u + kState8Block * 4, Codec<RG_F32, 4>::pack(b).v);
+  } else {
+    store4<RG_F32, NT>(vp + lane * 16, na, a);
+    store4<RG_F32, NT>(vp + (kState8Block * 4 + lane * 16), nb, b);
+  }
 }
 
 template <bool WRITE_CODES, bool NT>
-__global__ __launch_bounds__(kConvThreads) void state8_kernel(const State8Rec* recs, int tiles_per_chunk) {
-  const State8Rec r = recs[blockIdx.x / (unsigned)tiles_per_chunk];
+__global__ __launch_bounds__(kConvThreads) void state8_kernel(const State8Rec* recs) {
+  constexpr unsigned kTiles = (unsigned)(kState8ChunkElems / kConvTileElems);
+  const unsigned t = tile_of_block<kConvXcdRun>();
+  const State8Rec r = recs[t / kTiles];
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64u)), lane = (int)(threadIdx.x % 64u);
-  constexpr int kWaveElems = kConvTileElems / (kConvThreads / 64);
-  const int start = (int)(blockIdx.x % (unsigned)tiles_per_chunk) * kConvTileElems + wave * kWaveElems;
-  for (int b = start; b < start + kWaveElems && b < r.len; b += kState8Block) {
-    if (WRITE_CODES) {
-      if (r.root) quantize_block<true, NT>(r, b, lane);
-      else quantize_block<false, NT>(r, b, lane);
-    } else {
-      if (r.root) dequantize_block<true, NT>(r, b, lane);
-      else dequantize_block<false, NT>(r, b, lane);
-    }
+  const int start = (int)(t % kTiles) * kConvTileElems + wave * (2 * kState8Block);
+  if (start >= r.len) return;
+  const bool full = r.len - start >= 2 * kState8Block;
+#define RG_CONVERT(ROOT, FULL)                                        \
+  if ((r.root != 0) == ROOT && full == FULL) {                        \
+    if (WRITE_CODES) quantize_pair<ROOT, NT, FULL>(r, start, lane);   \
+    else dequantize_pair<ROOT, NT, FULL>(r, start, lane);             \
+    return;                                                           \
   }
+  RG_CONVERT(false, true)
+  RG_CONVERT(true, true)
+  RG_CONVERT(false, false)
+  RG_CONVERT(true, false)
+#undef RG_CONVERT
 }
 
 }  // namespace
@@ -340,8 +394,6 @@ struct rg_state8 {
   int64_t total_numel = 0;
   State8Rec* d_recs = nullptr;
 };
-
-constexpr int64_t kState8ChunkElems = 16384;
 
 RG_API int64_t rg_state8_num_scales(int64_t numel) { return numel < 0 ? -1 : (numel + kState8Block - 1) / kState8Block; }
 
@@ -434,16 +486,15 @@ static int launch_state8(const rg_state8* t, bool write_codes, void* stream, con
   }
   if (t->n_chunks == 0) return RG_OK;
   DeviceGuard guard(t->device);
-  const int tiles = (int)(kState8ChunkElems / kConvTileElems);
-  const dim3 grid((unsigned)(t->n_chunks * tiles)), block(kConvThreads);
+  const dim3 grid((unsigned)(t->n_chunks * (kState8ChunkElems / kConvTileElems))), block(kConvThreads);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const bool nt = t->total_numel * 5 > ((int64_t)256 << 20);
   if (write_codes) {
-    if (nt) hipLaunchKernelGGL((state8_kernel<true, true>), grid, block, 0, s, t->d_recs, tiles);
-    else hipLaunchKernelGGL((state8_kernel<true, false>), grid, block, 0, s, t->d_recs, tiles);
+    if (nt) hipLaunchKernelGGL((state8_kernel<true, true>), grid, block, 0, s, t->d_recs);
+    else hipLaunchKernelGGL((state8_kernel<true, false>), grid, block, 0, s, t->d_recs);
   } else {
-    if (nt) hipLaunchKernelGGL((state8_kernel<false, true>), grid, block, 0, s, t->d_recs, tiles);
-    else hipLaunchKernelGGL((state8_kernel<false, false>), grid, block, 0, s, t->d_recs, tiles);
+    if (nt) hipLaunchKernelGGL((state8_kernel<false, true>), grid, block, 0, s, t->d_recs);
+    else hipLaunchKernelGGL((state8_kernel<false, false>), grid, block, 0, s, t->d_recs);
   }
   RG_HIP(hipGetLastError());
   return RG_OK;
