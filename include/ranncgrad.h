@@ -355,7 +355,8 @@ int rg_sgd_step(rg_optim* opt, const rg_sgd_args* args, void* stream);
  * state1 = state2 = NULL: states stay where they are) and rg_optim_destroy take such a table; rg_sgd_step does not.
  *
  * Arithmetic of its Adam step, every operation in fp32 and rounded by itself (the division of the last line is within
- * 2 units in the last place), with g, p and the scalar factors as for rg_adam_step:
+ * 2 units in the last place; v does not underflow, it is carried times a power of two), with g, p and the scalar factors as
+ * for rg_adam_step:
  *   m = beta1 * m + (1 - beta1) * g
  *   v = beta2 * (r * r) + ((1 - beta2) * g) * g,   r = sqrt(v)
  *   p = p + ((-lr / (1 - beta1^step)) * m) / (r * (1 / sqrt(1 - beta2^step)) + eps)
@@ -370,9 +371,12 @@ int rg_optim_create_state8(rg_optim** out, int device, int n_tensors, void* cons
                            void* const* model_copy, const int64_t* numel, const int* grad_dtype, const int* copy_dtype);
 
 /* The same form from and to fp32, many tensors in one launch (a checkpoint in 32 bits is loaded or written).
- * root[i] != 0: values[i] is a second moment, stored as its root and read back as the root's square.  Quantizing
- * rounds to nearest, ties to even; what dequantizing gives quantizes to the same codes and scales again (roots: as long as the
- * squares are normal fp32 numbers).  A negative value under `root` counts as NaN.  The table borrows the addresses. */
+ * root[i] != 0: values[i] is a second moment, stored as its root and read back as the root's square; a negative one counts
+ * as NaN.  Quantizing rounds to nearest, ties to even.  What is read back quantizes to the same codes and scales again (roots:
+ * as long as the squares are normal fp32 numbers) if the block's largest code is 256's.  A quantized block always has that
+ * code.  So has one that a step wrote, but for about one in 2^21: 256 * x / s can come out a unit below 256 for the largest x,
+ * and a dither of zero then takes the number below.  Such a block is rounded to nearest once more.
+ * The table borrows the addresses. */
 typedef struct rg_state8 rg_state8;
 int rg_state8_create(rg_state8** out, int device, int n_tensors, void* const* codes, float* const* scales, float* const* values,
                      const int64_t* numel, const int* root);

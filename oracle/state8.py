@@ -76,16 +76,16 @@ def quantize(values: np.ndarray, root: bool) -> Tuple[np.ndarray, np.ndarray, np
     return codes.astype(np.uint8), s, np.abs(part - 0.5)
 
 
-def dither(numel: int, step: int, factor: int) -> np.ndarray:
-    """The 20-bit numbers of a tensor's elements at a step."""
-    i = np.arange(numel, dtype=np.uint64)
+def dither(numel: int, step: int, factor: int, first: int = 0) -> np.ndarray:
+    """The 20-bit numbers of a tensor's elements at a step, from its element ``first`` on."""
+    i = (np.arange(numel, dtype=np.uint64) + np.uint64(first)) & np.uint64(0xFFFFFFFF)
     u = (i * np.uint64(PLACE) + np.uint64(step % (1 << 32)) * np.uint64(factor)) & np.uint64(0xFFFFFFFF)
     return (u >> np.uint64(12)).astype(np.int64)
 
 
 def adam_step(p, g, codes1, scales1, codes2, scales2, step, lr, beta1, beta2, eps, weight_decay, decoupled=False,
-              maximize=False, grad_scale=1.0, coef=1.0) -> Dict[str, np.ndarray]:
-    """One step on a flat tensor, in float64 from the stored codes.  ``codes1`` / ``codes2`` of the result are what the
+              maximize=False, grad_scale=1.0, coef=1.0, first=0) -> Dict[str, np.ndarray]:
+    """One step on a flat tensor (or on whole blocks of one, from its element ``first`` on), in float64 from the stored codes.  ``codes1`` / ``codes2`` of the result are what the
     dither gives; ``sure1`` / ``sure2`` say where fp32 arithmetic cannot decide otherwise; ``p_tol`` bounds its error of p."""
     with np.errstate(all="ignore"):
         p = np.asarray(p, dtype=np.float64)
@@ -116,7 +116,7 @@ def adam_step(p, g, codes1, scales1, codes2, scales2, step, lr, beta1, beta2, ep
             s = scale_of(x)
             y = in_range(x, s, tag == "2")
             low, high, part = neighbours(y)
-            u = dither(x.size, step, factor)
+            u = dither(x.size, step, factor, first)
             up = part * 2.0 ** 20 + u >= 2.0 ** 20
             codes = np.where(up, high, low) | np.where(np.signbit(y), 0x80, 0)
             out["codes" + tag], out["scales" + tag] = codes.astype(np.uint8), s

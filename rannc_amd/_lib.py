@@ -428,6 +428,7 @@ class OptimTable:
         and of exp_avg_sq's root, and every 256 elements of a tensor have a float of each of the two."""
         n = len(numels)
         self._handle = _vp()
+        self._adam_key = self._adam_args = None
         self.n = n
         self.device = device
         a_cd = (C.c_int * max(n, 1))(*(copy_dtypes if copy_dtypes is not None else [RG_F32] * n))
@@ -459,8 +460,12 @@ class OptimTable:
     def adam_step(self, lr: float, beta1: float, beta2: float, eps: float, weight_decay: float, step: int,
                   decoupled: bool = False, maximize: bool = False, grad_scale: float = 1.0, gate: int = 0,
                   stream: int = 0) -> None:
-        a = AdamArgs(lr, beta1, beta2, eps, weight_decay, step, int(decoupled), int(maximize), grad_scale, gate or None)
-        check(lib.rg_adam_step(self._handle, C.byref(a), _vp(stream)))
+        key = (float(lr), float(beta1), float(beta2), float(eps), float(weight_decay), decoupled, maximize, float(grad_scale), gate)
+        if key != self._adam_key:       # filling the struct costs as much as the call: only the count changes with every step
+            self._adam_args = AdamArgs(lr, beta1, beta2, eps, weight_decay, step, int(decoupled), int(maximize), grad_scale, gate or None)
+            self._adam_key = key
+        self._adam_args.step = step
+        check(lib.rg_adam_step(self._handle, C.byref(self._adam_args), stream))
 
     def adam_step_clocked(self, clock_ptr: int, lr: float, beta1: float, beta2: float, eps: float, weight_decay: float,
                           decoupled: bool = False, maximize: bool = False, grad_scale: float = 1.0, gate: int = 0,

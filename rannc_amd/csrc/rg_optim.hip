@@ -461,7 +461,7 @@ static int create_table(rg_optim** out, int device, int n, const OptColumns& a, 
   o->n_chunks = o->chunk_begin[(size_t)n];
   int rc = check_rows(o, op);
   const int64_t tiles = (o->chunk_elems + kOptMinTileElems - 1) / kOptMinTileElems;
-  if (rc == RG_OK && o->n_chunks * tiles > 0x7fffffffLL) {
+  if (rc == RG_OK && !state8 && o->n_chunks * tiles > 0x7fffffffLL) {
     set_error("%s: %lld elements exceed one launch", op, (long long)o->total_numel);
     rc = RG_EINVAL;
   }
@@ -520,7 +520,7 @@ RG_API int rg_optim_destroy(rg_optim* o) {
 }
 
 RG_API int rg_optim_update_pointers(rg_optim* o, void* const* param, const void* const* grad, void* const* state1,
-                                    void* const* state2, void* const* model_copy, void* stream) {
+                                    void* const* state2, void* const* model_copy, void* stream) try {
   if (o == nullptr) {
     set_error("rg_optim_update_pointers: null table");
     return RG_EINVAL;
@@ -563,6 +563,9 @@ RG_API int rg_optim_update_pointers(rg_optim* o, void* const* param, const void*
   RG_HIP(hipEventRecord(o->stage_done[k], s));
   o->stage_used[k] = true;
   return RG_OK;
+} catch (const std::bad_alloc&) {
+  set_error("rg_optim_update_pointers: out of host memory");
+  return RG_ENOMEM;
 }
 
 template <int ALGO>
@@ -631,7 +634,7 @@ static int adam_step(rg_optim* o, const rg_adam_args* g, const rg_adam_clock* cl
     a.c.inv_bias2_sqrt = 1.0f / (float)sqrt(bias2);
     a.c.eps = (float)g->eps;
     DeviceGuard guard(o->device);
-    RG_HIP(launch_adam8(a, o->n_chunks, o->total_numel * 18 > ((int64_t)256 << 20),
+    RG_HIP(launch_adam8(a, o->n_chunks, streams(o->total_numel * 10),
                         reinterpret_cast<hipStream_t>(stream)));
     return RG_OK;
   }

@@ -104,8 +104,9 @@ __device__ __forceinline__ float sqrt_normal(float x) {
   return __builtin_fmaf(__builtin_fmaf(-s, s, x), 0.5f * y, s);
 }
 
-constexpr float kRootShift = 16777216.0f;                       // 2^24: the step's roots are carried times this, squares times 2^48
-constexpr float kSquareShift = 281474976710656.0f;
+// Squares are carried times 2^50 and roots times 2^25, so that every square that fp32 holds lies in sqrt_normal's range
+// (a product's factor is moved instead of the product, which costs nothing and changes no rounding).
+constexpr float kRootShift = 33554432.0f, kSquareShift = 1125899906842624.0f;
 
 // One block of 256 elements (fewer at a tensor's end) by one wavefront, four per lane.
 template <int G, int C, bool NT, bool FULL>
@@ -144,10 +145,11 @@ __device__ __forceinline__ void adam8_block(const Opt8ChunkRec& r, int start, in
     for (int j = 0; j < 4; ++j) g[j] = g[j] + c.weight_decay * p[j];
   }
   float root[4];
+  const float one_minus_beta2 = c.one_minus_beta2 * kSquareShift;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     m[j] = c.beta1 * m[j] + c.one_minus_beta1 * g[j];
-    root[j] = sqrt_normal(c.beta2 * (q[j] * q[j]) + (c.one_minus_beta2 * kSquareShift * g[j]) * g[j]);
+    root[j] = sqrt_normal(c.beta2 * (q[j] * q[j]) + (one_minus_beta2 * g[j]) * g[j]);
   }
   float top2 = __builtin_elementwise_maximum(maximum_abs3(root[0], root[1], root[2]), root[3]);
   const bool plain = __builtin_amdgcn_ballot_w64(top2 != top2) == 0;
@@ -155,8 +157,10 @@ __device__ __forceinline__ void adam8_block(const Opt8ChunkRec& r, int start, in
     top2 = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float old = q[j] * (1.0f / kRootShift);
-      root[j] = sqrtf(c.beta2 * (old * old) + (c.one_minus_beta2 * g[j]) * g[j]) * kRootShift;
+      const float square = c.beta2 * (q[j] * q[j]) + (one_minus_beta2 * g[j]) * g[j];
+      const float old = q[j] * (1.0f / kRootShift);      // the shift may have made it infinite
+      root[j] = square < __builtin_inff() ? sqrtf(square)
+                                          : sqrtf(c.beta2 * (old * old) + (c.one_minus_beta2 * g[j]) * g[j]) * kRootShift;
       top2 = __builtin_elementwise_maximum(top2, __builtin_fabsf(root[j]));
     }
   }
@@ -263,7 +267,7 @@ struct State8Rec {
 };
 static_assert(sizeof(State8Rec) == 32, "conversion record must stay 32 bytes");
 
-// The magnitudes to be stored: the values, or their roots (times 2^24).  `plain`: no root is zero or not a number.
+// The magnitudes to be stored: the values, or their roots (times kRootShift).  `plain`: no root is zero or not a number.
 template <bool ROOT> __device__ __forceinline__ bool stored_form(float (&x)[4], float& top) {
   if (!ROOT) {
     top = __builtin_elementwise_maximum(maximum_abs3(x[0], x[1], x[2]), __builtin_fabsf(x[3]));
@@ -377,11 +381,25 @@ __global__ __launch_bounds__(kConvThreads) void state8_kernel(const State8Rec* r
 
 }  // namespace
 
-hipError_t launch_adam8(const Adam8Args& a, int64_t n_chunks, bool streaming, hipStream_t stream) {
-  const dim3 grid((unsigned)(n_chunks * (kOpt8ChunkElems / kAdam8TileElems))), block(kAdam8Threads);
-  if (streaming) hipLaunchKernelGGL((adam8_kernel<true>), grid, block, 0, stream, a);
-  else hipLaunchKernelGGL((adam8_kernel<false>), grid, block, 0, stream, a);
-  return hipGetLastError();
+// A launch holds fewer than 2^32 threads: larger tables take several.
+constexpr int64_t kMaxBlocks = (int64_t)1 << 24;
+template <typename F> static hipError_t launch_in_parts(int64_t n_chunks, int64_t tiles_per_chunk, const F& launch) {
+  const int64_t most = kMaxBlocks / tiles_per_chunk;
+  for (int64_t at = 0; at < n_chunks; at += most) {
+    launch(at, (unsigned)(std::min(most, n_chunks - at) * tiles_per_chunk));
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+hipError_t launch_adam8(const Adam8Args& args, int64_t n_chunks, bool streaming, hipStream_t stream) {
+  return launch_in_parts(n_chunks, kOpt8ChunkElems / kAdam8TileElems, [&](int64_t at, unsigned blocks) {
+    Adam8Args a = args;
+    a.chunks += at;
+    if (streaming) hipLaunchKernelGGL((adam8_kernel<true>), dim3(blocks), dim3(kAdam8Threads), 0, stream, a);
+    else hipLaunchKernelGGL((adam8_kernel<false>), dim3(blocks), dim3(kAdam8Threads), 0, stream, a);
+  });
 }
 
 }  // namespace rg
@@ -407,8 +425,8 @@ RG_API int rg_state8_create(rg_state8** out, int device, int n, void* const* cod
   *out = nullptr;
   int64_t chunks = 0, total = 0;
   for (int i = 0; i < n; ++i) {
-    if (numel[i] < 0) {
-      set_error("rg_state8_create: tensor %d has a negative size", i);
+    if (numel[i] < 0 || numel[i] > kMaxTensorElems) {
+      set_error("rg_state8_create: tensor %d has %lld elements", i, (long long)numel[i]);
       return RG_EINVAL;
     }
     if (numel[i] == 0) continue;
@@ -420,16 +438,8 @@ RG_API int rg_state8_create(rg_state8** out, int device, int n, void* const* cod
     if (rc == RG_OK) rc = check_pointer(scales[i], 4, "scales", i);
     if (rc == RG_OK) rc = check_pointer(values[i], 4, "values", i);
     if (rc != RG_OK) return rc;
-    if (numel[i] > kMaxTensorElems) {
-      set_error("rg_state8_create: tensor %d has %lld elements", i, (long long)numel[i]);
-      return RG_EINVAL;
-    }
     chunks += (numel[i] + kState8ChunkElems - 1) / kState8ChunkElems;
     total += numel[i];
-    if (chunks * (kState8ChunkElems / kConvTileElems) > 0x7fffffffLL) {
-      set_error("rg_state8_create: %lld elements exceed one launch", (long long)total);
-      return RG_EINVAL;
-    }
   }
   rg_state8* t = new (std::nothrow) rg_state8;
   if (t == nullptr) {
@@ -486,17 +496,16 @@ static int launch_state8(const rg_state8* t, bool write_codes, void* stream, con
   }
   if (t->n_chunks == 0) return RG_OK;
   DeviceGuard guard(t->device);
-  const dim3 grid((unsigned)(t->n_chunks * (kState8ChunkElems / kConvTileElems))), block(kConvThreads);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const bool nt = t->total_numel * 5 > ((int64_t)256 << 20);
-  if (write_codes) {
-    if (nt) hipLaunchKernelGGL((state8_kernel<true, true>), grid, block, 0, s, t->d_recs);
-    else hipLaunchKernelGGL((state8_kernel<true, false>), grid, block, 0, s, t->d_recs);
-  } else {
-    if (nt) hipLaunchKernelGGL((state8_kernel<false, true>), grid, block, 0, s, t->d_recs);
-    else hipLaunchKernelGGL((state8_kernel<false, false>), grid, block, 0, s, t->d_recs);
-  }
-  RG_HIP(hipGetLastError());
+  const bool nt = streams(t->total_numel * 5);
+  RG_HIP(launch_in_parts(t->n_chunks, kState8ChunkElems / kConvTileElems, [&](int64_t at, unsigned blocks) {
+    const dim3 grid(blocks), block(kConvThreads);
+    const State8Rec* recs = t->d_recs + at;
+    if (write_codes && nt) hipLaunchKernelGGL((state8_kernel<true, true>), grid, block, 0, s, recs);
+    else if (write_codes) hipLaunchKernelGGL((state8_kernel<true, false>), grid, block, 0, s, recs);
+    else if (nt) hipLaunchKernelGGL((state8_kernel<false, true>), grid, block, 0, s, recs);
+    else hipLaunchKernelGGL((state8_kernel<false, false>), grid, block, 0, s, recs);
+  }));
   return RG_OK;
 }
 

@@ -324,7 +324,8 @@ class FusedAdam(_FusedBase):
         so that a run can be repeated bit for bit.  ``state[p]`` then has the codes under ``exp_avg`` / ``exp_avg_sq``
         and the scales under ``exp_avg_scale`` / ``exp_avg_sq_scale``; ``state_dict()`` gives, and ``load_state_dict()``
         takes, the float32 moments of ``torch.optim.Adam`` - converted on the GPU, which holds both forms meanwhile.  What
-        ``state_dict()`` gave loads back as the same codes and scales.  Everything else works as with 32 bits.
+        ``state_dict()`` gave loads back as the same codes and scales (but for about one block in two million, see
+        ``rg_state8_quantize``).  Everything else works as with 32 bits.
 
         ``capturable``: as in ``torch.optim.Adam`` - the step count lives on the device (``state["step"]`` is a
         0-dim float32 GPU tensor), nothing about a step is decided on the host, and ``step()`` may be recorded in
@@ -387,7 +388,7 @@ class FusedAdam(_FusedBase):
         """Between the 8-bit states of ``params`` and the float32 moments in ``entries``."""
         by_device: Dict[torch.device, List[int]] = {}
         for i, p in enumerate(params):
-            by_device.setdefault(p.device, []).append(i)
+            by_device.setdefault(self.state[p]["exp_avg"].device, []).append(i)
         for rows in by_device.values():
             values, codes, scales, roots = [], [], [], []
             for name in ("exp_avg", "exp_avg_sq"):
@@ -413,8 +414,8 @@ class FusedAdam(_FusedBase):
         entries = []
         for i, p in held:
             entry = {k: v.clone() if torch.is_tensor(v) else v for k, v in packed["state"][i].items() if not k.startswith("exp_avg")}
-            entry["exp_avg"] = torch.empty(p.shape, dtype=torch.float32, device=p.device)
-            entry["exp_avg_sq"] = torch.empty(p.shape, dtype=torch.float32, device=p.device)
+            for name in ("exp_avg", "exp_avg_sq"):        # on the GPU, also where the parameter has gone to the host
+                entry[name] = torch.empty(p.shape, dtype=torch.float32, device=self.state[p][name].device)
             entries.append(entry)
         self._convert_moments([p for _, p in held], entries, to_codes=False)
         packed["state"] = dict(packed["state"])

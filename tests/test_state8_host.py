@@ -79,7 +79,7 @@ def test_table_refusals_come_before_the_device():
     ok = dict(device=0, codes=[0x1000], scales=[0x2000], values=[0x3000], numels=[10], roots=[False])
     for bad, match in ((dict(codes=[0x1001]), "aligned"), (dict(scales=[0x2002]), "aligned"), (dict(values=[0x3002]), "aligned"),
                        (dict(codes=[0]), "lacks"), (dict(scales=[0]), "lacks"), (dict(values=[0]), "lacks"),
-                       (dict(numels=[-1]), "negative"), (dict(numels=[2 ** 45]), "elements"), (dict(numels=[2 ** 44]), "one launch"),
+                       (dict(numels=[-1]), "elements"), (dict(numels=[2 ** 45]), "elements"),
                        (dict(codes=[]), "length")):
         with pytest.raises(ValueError, match=match):
             _lib.State8Table(**{**ok, **bad})
@@ -95,7 +95,7 @@ def test_optim_table_refusals_come_before_the_device():
                        (dict(scales2=[0]), "scales"), (dict(scales1=None), "bad arguments"), (dict(scales2=None), "bad arguments"),
                        (dict(state1=None), "bad arguments"), (dict(state2=[0]), "state pointer"), (dict(params=[0x1002]), "aligned"),
                        (dict(grads=[0]), "gradient"), (dict(numels=[-1]), "bad size"), (dict(numels=[2 ** 45]), "bad size"),
-                       (dict(numels=[2 ** 44]), "one launch"), (dict(grad_dtypes=[7]), "dtype")):
+                       (dict(grad_dtypes=[7]), "dtype")):
         with pytest.raises(ValueError, match=match):
             make(**bad)
 
