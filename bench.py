@@ -32,7 +32,8 @@ FUSED_OPS = ("fused_step", "fused_step_noclip", "fused_step_noclip_2pass", "over
              "consolidate", "zero_staging_pack")
 C5_OPS = ("c5_unflatten", "c5_master_cast", "c5_copy_back", "c5_repack")
 OPTIM_OPS = ("adam", "sgd", "adam_from_model_grads")
-ALL_OPS = ("all",) + FUSED_OPS + C5_OPS + OPTIM_OPS + ("api_step", "graph_step", "ceilings")
+STATE8_OPS = ("adam_state8", "quantize_states", "dequantize_states")      # by --op only: no part of the default line
+ALL_OPS = ("all",) + FUSED_OPS + C5_OPS + OPTIM_OPS + STATE8_OPS + ("api_step", "graph_step", "ceilings")
 
 
 def parse_args():
@@ -627,6 +628,48 @@ def bench_optimizer(args, key, torch, dev) -> dict:
     return out
 
 
+def bench_state8(args, key, torch, dev) -> dict:
+    """Optimizer states in 8 bits over the workload's tensors: the Adam step as ``adam`` has it (fp32 masters and master
+    gradients, model copy written), or both moments' conversion from fp32 or back."""
+    from rannc_amd.fused_optim import FusedAdam
+    from rannc_amd.multi_tensor import State8Plan
+    from rannc_amd.workloads import step_config
+
+    cfg = step_config(key)
+    shapes = [sh for _, sh in cfg.params]
+    copy_dt = torch.float16 if cfg.grad_dtype == "f16" else torch.bfloat16
+    gen = torch.Generator(device=dev).manual_seed(args.seed)
+    params = [torch.randn(sh, device=dev, generator=gen) for sh in shapes]
+    n = sum(p.numel() for p in params)
+    for p in params:
+        p.grad = torch.randn(p.shape, device=dev, generator=gen) * 1e-2
+    opt = FusedAdam(params, lr=1e-3, state_bits=8)
+    opt.set_model_copies(params, [torch.zeros(sh, device=dev, dtype=copy_dt) for sh in shapes])
+    opt.step()
+    scales = opt.state_buffers()["exp_avg_scale"].numel()
+    plan = None
+    if args.op == "adam_state8":
+        step, step_bytes, kernel = opt.step, n * (8 + 4 + 4 + 2) + 16 * scales, "adam8_kernel"
+    else:
+        held = opt.state_dict()["state"]
+        names = ("exp_avg", "exp_avg_sq")
+        plan = State8Plan([held[i][k] for k in names for i in range(len(params))], [opt.state[p][k] for k in names for p in params],
+                          [opt.state[p][k + "_scale"] for k in names for p in params], [k == "exp_avg_sq" for k in names for _ in params])
+        step = plan.quantize if args.op == "quantize_states" else plan.dequantize
+        step_bytes, kernel = 2 * (5 * n + 4 * scales), "state8_kernel"
+    step_s, launch_s = timed(step, args.steps, args.warmup, 20)
+    return {
+        "metric": f"achieved HBM GB/s for the multi-tensor {args.op} pass",
+        "value": round(step_bytes / step_s / 1e9, 1), "unit": "GB/s", "n_gpus": 1, "steps": args.steps,
+        "warmup": args.warmup, "ms_per_step": round(step_s * 1e3, 4), "higher_is_better": True, "scaling": "weak",
+        "vs_baseline": None, "dtype": "f32", "data": "synthetic",
+        "config": {"workload": cfg.key, "op": args.op, "tensors": len(params), "elements": n, "model_copy_dtype": str(copy_dt),
+                   "seed": args.seed},
+        "pct_of_hbm_peak": round(100.0 * step_bytes / step_s / 1e9 / HBM_PEAK_GBPS, 2),
+        "roofline": roofline(kernel, step_bytes, launch_s, measured_traffic(args.op, cfg.key, kernel)),
+    }
+
+
 def cpu_baseline_optimizer(op: str, shapes, seed: int, budget_s: float, bytes_per_elem: int) -> dict:
     """torch.optim's op sequence (the oracle restates it; bit-identical to the library) on the
     host cores, over as many leading tensors of the workload as fit the time budget."""
@@ -927,6 +970,10 @@ def main() -> int:
     everything = args.op in (None, "all") and args.workload is None
     if args.op in OPTIM_OPS:
         print(json.dumps(bench_optimizer(args, args.workload or "c2_bert_large", torch, dev)), flush=True)
+        return 0
+
+    if args.op in STATE8_OPS:
+        print(json.dumps(bench_state8(args, args.workload or "c2_bert_large", torch, dev)), flush=True)
         return 0
 
     if args.op == "graph_step":

@@ -336,7 +336,8 @@ class FusedAdam(_FusedBase):
         What a capture freezes: ``lr``, ``betas``, ``eps``, ``weight_decay`` and ``maximize`` of every group, and
         ``grad_scale`` when it is passed by value, are kernel arguments and so become part of the recorded graph -
         changing ``param_groups[i]["lr"]`` afterwards affects eager steps only, a replayed graph keeps the values
-        of the capture (record a new graph after a learning-rate change).  What a replay does follow, because it
+        of the capture (record a new graph after a learning-rate change, and after ``load_state_dict``, which makes new state
+        tensors).  What a replay does follow, because it
         is read from device memory: the step count and its bias corrections, the gate (clip coefficient, skip)
         and, with ``grad_scale_ptr``, 1 / loss scale."""
         if lr < 0 or eps < 0 or not 0 <= betas[0] < 1 or not 0 <= betas[1] < 1 or weight_decay < 0:
@@ -525,12 +526,15 @@ class FusedAdam(_FusedBase):
             step_tensors = []
             grad_of: Dict[int, torch.Tensor] = {}
             fresh = []
-            for p in group["params"]:
+            found = []
+            for p in group["params"]:            # all of them are looked at before any count moves
                 g = self._grad_of(p)
                 if g is None:
                     continue
                 self._check_param(p, g)
+                found.append(p)
                 grad_of[id(p)] = g
+            for p in found:
                 st = self.state[p]
                 if "exp_avg" not in st:
                     st.setdefault("step", torch.tensor(0.0, dtype=torch.float32))

@@ -249,6 +249,8 @@ class State8Plan:
 def allocate_state8(like: Sequence[torch.Tensor]) -> Tuple[List[torch.Tensor], List[torch.Tensor], torch.Tensor, torch.Tensor]:
     """Zeroed 8-bit states for tensors on one GPU: ``(codes, scales, all codes, all scales)``.  The first two are views, of
     the given tensors' shapes and one scale per block, into the flat last two, where each tensor starts at a whole block."""
+    if not like:
+        raise ValueError("allocate_state8: no tensors")
     numels = [t.numel() for t in like]
     blocks = [_lib.state8_num_scales(n) for n in numels]
     device = like[0].device

@@ -219,6 +219,24 @@ def test_parameters_on_the_host_between_steps():
     _same_moments(a.state_dict()["state"], b.state_dict()["state"])
 
 
+@pytest.mark.parametrize("bits", [8, 32])
+def test_refused_step_counts_for_nothing(bits):
+    params = [torch.nn.Parameter(torch.ones(10, device=DEV)), torch.nn.Parameter(torch.zeros(4, 6, device=DEV).t())]
+    other = torch.nn.Parameter(torch.ones(10, device=DEV))
+    opt, ref = FusedAdam(params, state_bits=bits), FusedAdam([other], state_bits=bits)
+    params[1].grad = torch.ones(6, 4, device=DEV)
+    for p in (params[0], other):
+        p.grad = torch.full((10,), 0.25, device=DEV)
+    for _ in range(2):
+        with pytest.raises(ValueError, match="contiguous"):
+            opt.step()
+    params[1].grad = None
+    for step in range(3):
+        opt.step()
+        ref.step()
+        assert torch.equal(params[0], other) and float(opt.state[params[0]]["step"]) == step + 1
+
+
 def test_refused_step_leaves_no_half_made_state():
     params = [torch.nn.Parameter(torch.zeros(10, device=DEV)), torch.nn.Parameter(torch.zeros(4, 6, device=DEV).t())]
     opt = FusedAdam(params, state_bits=8)

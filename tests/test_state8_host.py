@@ -7,7 +7,7 @@ import torch
 from oracle import state8 as oracle
 from rannc_amd import _lib
 from rannc_amd.fused_optim import FusedAdam, FusedAdamW
-from rannc_amd.multi_tensor import State8Plan
+from rannc_amd.multi_tensor import State8Plan, allocate_state8
 
 
 def test_grid_is_e4m3():
@@ -127,6 +127,15 @@ def test_plan_refuses_what_is_not_on_a_gpu():
         State8Plan([v], [], [torch.zeros(1)])
     with pytest.raises(ValueError, match="length"):
         State8Plan([v], [torch.zeros(10, dtype=torch.float8_e4m3fn)], [torch.zeros(1)], root=[True, False])
+
+
+def test_allocation_layout():
+    codes, scales, all_codes, all_scales = allocate_state8([torch.zeros(3, 100), torch.zeros(0), torch.zeros(256), torch.zeros(1)])
+    assert [tuple(c.shape) for c in codes] == [(3, 100), (0,), (256,), (1,)] and [s.numel() for s in scales] == [2, 0, 1, 1]
+    assert all_codes.numel() == 1024 and all_codes.dtype == torch.float8_e4m3fn and all_scales.numel() == 4
+    assert [c.storage_offset() for c in codes] == [0, 512, 512, 768] and [s.storage_offset() for s in scales] == [0, 2, 2, 3]
+    with pytest.raises(ValueError, match="no tensors"):
+        allocate_state8([])
 
 
 @pytest.mark.parametrize("cls", [FusedAdam, FusedAdamW])
