@@ -26,7 +26,7 @@ __device__ __forceinline__ uint32_t magnitude_bits(float x) { return __float_as_
 
 // The largest of two numbers per lane, both at once: lanes 0-31 get the largest `a`, lanes 32-63 the largest `b` (all 64
 // lanes active).  The halves trade places (a's upper for b's lower), then the two rows of 16 lanes of each half, then
-// rotations within a row: 8 instructions, where two reductions of 64 lanes one after the other take 22.  On magnitudes'
+// rotations within a row: 9 instructions, where two reductions of 64 lanes one after the other take 16 and more.  On magnitudes'
 // bits the order is that of the numbers with infinity above them and NaN above that, so neither is lost on the way.
 template <int N> __device__ __forceinline__ uint32_t max_row_ror(uint32_t x) {
   const uint32_t y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x120 + N, 0xf, 0xf, true);

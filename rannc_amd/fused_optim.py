@@ -319,7 +319,7 @@ class FusedAdam(_FusedBase):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, maximize=False,
                  capturable=False, state_bits=32):
         """``state_bits=8``: both moments are held in 8 bits (``ranncgrad.h``, "optimizer states in 8 bits"): a byte an
-        element and a float32 scale for every 256 of them, a quarter of the memory and of the traffic.  The exp_avg_sq half is
+        element and a float32 scale for every 256 of them, a quarter of the moments' memory and traffic.  exp_avg_sq is
         held as its root, and a step rounds with a dither that depends on the step count and the element's place alone,
         so that a run can be repeated bit for bit.  ``state[p]`` then has the codes under ``exp_avg`` / ``exp_avg_sq``
         and the scales under ``exp_avg_scale`` / ``exp_avg_sq_scale``; ``state_dict()`` gives, and ``load_state_dict()``
@@ -350,8 +350,8 @@ class FusedAdam(_FusedBase):
         self._clocks: Dict[int, torch.Tensor] = {}       # group index -> its rg_adam_clock (8 float32 words on the device)
         self._buffers8: Dict[int, List[Dict[str, torch.Tensor]]] = {}      # group index -> the buffers its 8-bit states lie in
 
-    def _make_moments(self, gi: int, params: List[torch.Tensor]) -> None:
-        """Zero moments for ``params`` of one group (``step`` is the caller's)."""
+    def _make_moments(self, gi: int, params: List[torch.Tensor], loaded: Optional[List[Dict]] = None) -> None:
+        """Moments for ``params`` of one group (``step`` is the caller's): zeros, or in 8 bits what ``loaded`` holds in 32."""
         if self.state_bits == 32:
             for p in params:
                 self.state[p]["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
@@ -360,10 +360,15 @@ class FusedAdam(_FusedBase):
         if not params:
             return
         buffers: Dict[str, torch.Tensor] = {}
+        made: List[Dict[str, torch.Tensor]] = [{} for _ in params]
         for name in ("exp_avg", "exp_avg_sq"):
             codes, scales, buffers[name], buffers[name + "_scale"] = allocate_state8(params)
-            for p, c, s in zip(params, codes, scales):
-                self.state[p][name], self.state[p][name + "_scale"] = c, s
+            for entry, c, s in zip(made, codes, scales):
+                entry[name], entry[name + "_scale"] = c, s
+        if loaded is not None:
+            self._convert_moments(made, loaded, to_codes=True)
+        for p, entry in zip(params, made):       # only now: whatever failed before has left the states as they were
+            self.state[p].update(entry)
         self._buffers8.setdefault(gi, []).append(buffers)
 
     def _moments(self, params: List[torch.Tensor]):
@@ -385,17 +390,18 @@ class FusedAdam(_FusedBase):
                                "state_buffers: the group's states came in more than one step and lie in several buffers")
         return dict(held[0])
 
-    def _convert_moments(self, params: List[torch.Tensor], entries: List[Dict], to_codes: bool) -> None:
-        """Between the 8-bit states of ``params`` and the float32 moments in ``entries``."""
+    @staticmethod
+    def _convert_moments(held: List[Dict], entries: List[Dict], to_codes: bool) -> None:
+        """Between the 8-bit states in ``held`` and the float32 moments in ``entries``."""
         by_device: Dict[torch.device, List[int]] = {}
-        for i, p in enumerate(params):
-            by_device.setdefault(self.state[p]["exp_avg"].device, []).append(i)
+        for i, st in enumerate(held):
+            by_device.setdefault(st["exp_avg"].device, []).append(i)
         for rows in by_device.values():
             values, codes, scales, roots = [], [], [], []
             for name in ("exp_avg", "exp_avg_sq"):
                 values += [entries[i][name] for i in rows]
-                codes += [self.state[params[i]][name] for i in rows]
-                scales += [self.state[params[i]][name + "_scale"] for i in rows]
+                codes += [held[i][name] for i in rows]
+                scales += [held[i][name + "_scale"] for i in rows]
                 roots += [name == "exp_avg_sq"] * len(rows)
             plan = State8Plan(values, codes, scales, roots)
             if to_codes:
@@ -418,12 +424,15 @@ class FusedAdam(_FusedBase):
             for name in ("exp_avg", "exp_avg_sq"):        # on the GPU, also where the parameter has gone to the host
                 entry[name] = torch.empty(p.shape, dtype=torch.float32, device=self.state[p][name].device)
             entries.append(entry)
-        self._convert_moments([p for _, p in held], entries, to_codes=False)
+        self._convert_moments([self.state[p] for _, p in held], entries, to_codes=False)
         packed["state"] = dict(packed["state"])
         packed["state"].update((i, entry) for (i, _), entry in zip(held, entries))
         return packed
 
     def load_state_dict(self, state_dict) -> None:
+        if any("exp_avg_scale" in st for st in state_dict.get("state", {}).values()):
+            raise ValueError("the state dict holds 8-bit codes and scales; states are loaded from the float32 moments that "
+                             "state_dict() gives")
         super().load_state_dict(state_dict)
         self._clocks.clear()          # re-seeded from the loaded ``step`` values by the next step
         if self.state_bits == 32:
@@ -446,8 +455,7 @@ class FusedAdam(_FusedBase):
             if st["exp_avg"].numel() != p.numel() or st["exp_avg_sq"].numel() != p.numel():
                 raise ValueError("loaded moments differ in size from their parameter")
             entries.append({k: st[k].to(p.device, torch.float32).contiguous() for k in ("exp_avg", "exp_avg_sq")})
-        self._make_moments(gi, loaded)
-        self._convert_moments(loaded, entries, to_codes=True)
+        self._make_moments(gi, loaded, entries)
 
     def _capturable_step(self, gi: int, group) -> None:
         """One group's step with its count on the device: advance the clock (one thread), then the update kernel."""

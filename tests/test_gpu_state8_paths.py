@@ -253,6 +253,29 @@ def test_refused_step_leaves_no_half_made_state():
         opt.load_state_dict(sd)
 
 
+def test_failed_conversion_keeps_the_loaded_moments(monkeypatch):
+    """What a conversion that fails leaves behind is the float32 moments, not zeros."""
+    def trained(opt, p):
+        p.grad = torch.randn(700, generator=torch.Generator().manual_seed(1)).to(DEV)
+        opt.step()
+        return opt.state_dict()
+
+    p, q = (torch.nn.Parameter(torch.ones(700, device=DEV)) for _ in range(2))
+    sd = trained(FusedAdam([p], state_bits=8), p)
+    opt = FusedAdam([q], state_bits=8)
+    with monkeypatch.context() as m:
+        m.setattr(State8Plan, "quantize", lambda self: (_ for _ in ()).throw(MemoryError("no memory")))
+        with pytest.raises(MemoryError):
+            opt.load_state_dict(sd)
+    assert opt.state[q]["exp_avg"].dtype == torch.float32 and torch.equal(opt.state[q]["exp_avg"], sd["state"][0]["exp_avg"])
+    q.grad = torch.zeros(700, device=DEV)
+    opt.step()                                     # converts now
+    assert opt.state[q]["exp_avg"].dtype == torch.float8_e4m3fn and float(opt.state[q]["step"]) == 2
+    back = opt.state_dict()["state"][0]["exp_avg"]
+    want = 0.9 * sd["state"][0]["exp_avg"]
+    assert bool(((back - want).abs() <= want.abs() / 8 * (1 + 1e-5) + want.abs().max() * 2.0 ** -17).all())
+
+
 def test_learning_rate_as_a_tensor_and_by_a_schedule():
     p, q = (torch.nn.Parameter(torch.ones(300, device=DEV)) for _ in range(2))
     lr = torch.tensor(0.1)

@@ -154,3 +154,15 @@ def test_optimizer_arguments(cls):
     p[0].grad = torch.zeros(4)
     with pytest.raises(ValueError, match="GPU"):
         opt.step()
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_raw_codes_are_not_loaded(bits):
+    p = [torch.zeros(4)]
+    opt = FusedAdam(p, state_bits=bits)
+    sd = opt.state_dict()
+    codes, scales, _, _ = allocate_state8(p)
+    sd["state"] = {0: {"step": torch.tensor(1.0), "exp_avg": codes[0], "exp_avg_scale": scales[0], "exp_avg_sq": codes[0], "exp_avg_sq_scale": scales[0]}}
+    with pytest.raises(ValueError, match="8-bit codes"):
+        opt.load_state_dict(sd)
+    assert not opt.state
