@@ -139,20 +139,14 @@ __device__ __forceinline__ void adam8_block(const Opt8ChunkRec& r, int start, in
   load4<RG_F32, NT>(pp + lane * 16, n, p);
   load4<G, NT>(gp + lane * (4 * GS), n, g);
   const uint32_t w1 = load_codes4<NT>(c1 + lane * 4, n), w2 = load_codes4<NT>(c2 + lane * 4, n);
-  const float s1_old = r.scales1[block], s2_old = r.scales2[block];
+  const float s1_old = load_scale(r.scales1 + block), s2_old = load_scale(r.scales2 + block);
   decode(w1, s1_old * 0.00390625f, m);                                       // s / 256
   decode(w2, s2_old * (0.00390625f * kRootShift), q);
-  if (c.grad_scale != 1.0f) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) g[j] = g[j] * c.grad_scale;
-  }
-  if (coef != 1.0f) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) g[j] = g[j] * coef;
-  }
-  if (c.param_mul != 1.0f) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) p[j] = p[j] * c.param_mul;
+  for (int j = 0; j < 4; ++j) {        // x * 1 is x: no branch needed
+    g[j] = g[j] * c.grad_scale;
+    g[j] = g[j] * coef;
+    p[j] = p[j] * c.param_mul;
   }
   if (c.weight_decay != 0.0f) {
 #pragma unroll
@@ -353,7 +347,7 @@ __device__ __forceinline__ void dequantize_pair(const State8Rec& r, int start, i
   const uint32_t wa = load_codes4<NT>(cp + lane * 4, na), wb = load_codes4<NT>(cp + (kState8Block + lane * 4), nb);
   const int block = start / kState8Block;
   const bool second = FULL || r.len - start > kState8Block;
-  const float sa = r.scales[block], sb = second ? r.scales[block + 1] : 0.0f;
+  const float sa = load_scale(r.scales + block), sb = second ? load_scale(r.scales + block + 1) : 0.0f;
   float a[4], b[4];
   decode(wa, sa * 0.00390625f, a);
   decode(wb, sb * 0.00390625f, b);
