@@ -211,7 +211,8 @@ class State8Plan:
 
     ``codes[i]`` is a float8_e4m3fn tensor of ``values[i]``'s size, ``scales[i]`` a float32 one with an element for every
     256 of it (``allocate_state8`` makes both).  With ``root`` (one bool, or one per tensor) the values are second moments:
-    stored as their roots, read back as the roots' squares.  All tensors must be contiguous and on one GPU."""
+    stored as their roots, read back as the roots' squares.  All tensors must be contiguous, on one GPU and apart in memory.
+    The launches go to the current stream."""
 
     def __init__(self, values: Sequence[torch.Tensor], codes: Sequence[torch.Tensor], scales: Sequence[torch.Tensor],
                  root: Union[bool, Sequence[bool]] = False):
@@ -221,8 +222,9 @@ class State8Plan:
             raise ValueError("values, codes, scales and root differ in length")
         self.device = values[0].device if n else torch.device("cuda", torch.cuda.current_device())
         for i, (v, c, s) in enumerate(zip(values, codes, scales)):
-            for what, t, dtype, numel in (("values", v, torch.float32, v.numel()), ("codes", c, torch.float8_e4m3fn, v.numel()),
-                                          ("scales", s, torch.float32, _lib.state8_num_scales(v.numel()))):
+            n_i = v.numel()
+            for what, t, dtype, numel in (("values", v, torch.float32, n_i), ("codes", c, torch.float8_e4m3fn, n_i),
+                                          ("scales", s, torch.float32, -(-n_i // _lib.STATE8_BLOCK))):
                 _check_tensor(t, self.device, what, i)
                 if t.dtype != dtype:
                     raise ValueError(f"{what}[{i}] is {t.dtype}, expected {dtype}")
@@ -252,16 +254,13 @@ def allocate_state8(like: Sequence[torch.Tensor]) -> Tuple[List[torch.Tensor], L
     if not like:
         raise ValueError("allocate_state8: no tensors")
     numels = [t.numel() for t in like]
-    blocks = [_lib.state8_num_scales(n) for n in numels]
+    blocks = [-(-n // _lib.STATE8_BLOCK) for n in numels]
     device = like[0].device
     all_codes = torch.zeros(sum(blocks) * _lib.STATE8_BLOCK, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
     all_scales = torch.zeros(sum(blocks), dtype=torch.float32, device=device)
-    codes, scales, at = [], [], 0
-    for t, n, b in zip(like, numels, blocks):
-        codes.append(all_codes[at * _lib.STATE8_BLOCK:at * _lib.STATE8_BLOCK + n].view(t.shape))
-        scales.append(all_scales[at:at + b])
-        at += b
-    return codes, scales, all_codes, all_scales
+    whole = all_codes.split([b * _lib.STATE8_BLOCK for b in blocks])
+    codes = [(c if c.numel() == n else c[:n]).view(t.shape) for c, n, t in zip(whole, numels, like)]
+    return codes, list(all_scales.split(blocks)), all_codes, all_scales
 
 
 def fill_zero_(t: torch.Tensor) -> torch.Tensor:
