@@ -12,6 +12,7 @@
 #include <algorithm>
 #include <map>
 #include <memory>
+#include <string>
 #include <unordered_map>
 
 #include "rg_bind.h"
@@ -19,6 +20,14 @@
 using namespace rgbind;
 
 namespace {
+
+// Whether a gradient can be a row of an optimizer table as it is, and its address appended if so.
+bool append_address(const at::Tensor& g, at::ScalarType dtype, std::string& out) {
+  if (!g.defined() || g.layout() != at::kStrided || g.scalar_type() != dtype || !g.is_contiguous()) return false;
+  const uintptr_t address = reinterpret_cast<uintptr_t>(g.numel() ? g.const_data_ptr() : nullptr);
+  out.append(reinterpret_cast<const char*>(&address), sizeof(address));
+  return true;
+}
 
 // ------------------------------------------------------------------------------------------------ TensorList
 
@@ -46,6 +55,14 @@ class TensorList {
   void set_grads(const TensorList& views) {
     if (views.size() != t_.size()) throw std::invalid_argument("set_grads: the lists differ in length");
     for (size_t i = 0; i < t_.size(); ++i) t_[i].mutable_grad() = views.t_[i];
+  }
+  // The addresses of all gradients, one machine word each; None unless every tensor has a contiguous one of `dtype`.
+  py::object grad_addresses(at::ScalarType dtype) const {
+    std::string out;
+    out.reserve(t_.size() * sizeof(uintptr_t));
+    for (const at::Tensor& t : t_)
+      if (!t.defined() || !append_address(t.grad(), dtype, out)) return py::none();
+    return py::bytes(out);
   }
   void clear_grads() {
     for (at::Tensor& t : t_)
@@ -726,6 +743,16 @@ void bind_registry(py::module_& m) {
   });
   m.def("get_amp_master_param", [](long model_param_id) { return global_storage()->get_amp_master_param_tensor(model_param_id); });
 
+  // TensorList.grad_addresses for gradients that are given themselves (None among them: no gradient)
+  m.def("tensor_addresses", [](const py::list& tensors, const py::object& dtype) -> py::object {
+    const at::ScalarType dt = torch::python::detail::py_object_to_dtype(dtype);
+    std::string out;
+    out.reserve(tensors.size() * sizeof(uintptr_t));
+    for (const py::handle& o : tensors)
+      if (!append_address(tensor_or_undefined(o, "tensor_addresses"), dt, out)) return py::none();
+    return py::bytes(out);
+  });
+
   py::class_<TensorList, std::shared_ptr<TensorList>>(m, "TensorList")
       .def(py::init<const py::object&>(), py::arg("tensors"))
       .def("__len__", &TensorList::size)
@@ -737,6 +764,9 @@ void bind_registry(py::module_& m) {
              return ok ? n : -1;
            }, "number of tensors with a gradient; -1 unless each of those gradients is a contiguous GPU tensor of `dtype` and of its owner's size")
       .def("grads", &TensorList::grads)
+      .def("grad_addresses", [](const TensorList& l, const py::object& dtype) {
+             return l.grad_addresses(torch::python::detail::py_object_to_dtype(dtype));
+           }, "the gradients' addresses as packed machine words; None unless every tensor has a contiguous gradient of `dtype`")
       .def("set_grads", &TensorList::set_grads)
       .def("clear_grads", &TensorList::clear_grads);
 

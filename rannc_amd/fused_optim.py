@@ -11,6 +11,7 @@ them unchanged.  There is no CPU path: parameters must live on the GPU.
 """
 from __future__ import annotations
 
+from array import array
 from typing import Dict, List, Optional, Tuple
 
 import torch
@@ -25,7 +26,21 @@ except ImportError:
 
 
 _data_ptr = torch.Tensor.data_ptr
-_is_contiguous = torch.Tensor.is_contiguous
+
+
+def _packed(tensors) -> bytes:
+    """Their addresses, one machine word each."""
+    return array("Q", map(_data_ptr, tensors)).tobytes()
+
+
+def _addresses(grads: List[Optional[torch.Tensor]], dtype: torch.dtype) -> Optional[bytes]:
+    """``_packed(grads)``; None unless every gradient is there, contiguous and of ``dtype``."""
+    if _native is not None:
+        return _native.tensor_addresses(grads, dtype)
+    for g in grads:
+        if g is None or g.dtype != dtype or g.layout != torch.strided or not g.is_contiguous():
+            return None
+    return _packed(grads)
 
 
 def _own_step(impl):
@@ -150,10 +165,18 @@ class _FusedBase(torch.optim.Optimizer):
         every tensor again and pushes all addresses to the device."""
         self._steady.clear()
         self._tables.clear()
+        self._native_lists.clear()
 
-    def _steady_grads(self, gi: int, group) -> Optional[Tuple["_Steady", List[torch.Tensor]]]:
-        """The group's steady-state record and this step's gradients, or None when anything about the group
-        differs from the step that made the record (then the full path runs and makes a new one)."""
+    def _native_list(self, gi: int, params):
+        """The compiled module's list of a group's parameters."""
+        known = self._native_lists.get(gi)
+        if known is None or known[0] is not params or known[1] != len(params):
+            known = self._native_lists[gi] = (params, len(params), _native.TensorList(params))
+        return known[2]
+
+    def _steady_grads(self, gi: int, group) -> Optional["_Steady"]:
+        """The group's steady-state record, its table pointing at this step's gradients, or None when anything about
+        the group differs from the step that made the record (then the full path runs and makes a new one)."""
         st = self._steady.get(gi)
         params = group["params"]
         if st is None or st.params_obj is not params or len(params) != st.n:
@@ -172,36 +195,31 @@ class _FusedBase(torch.optim.Optimizer):
                     hit = self._tables.get(st.key)
                     if hit is not None and hit[0] is st.table:
                         self._tables[st.key] = (hit[0], None, hit[2])
-                return st, None
+                return st
             self._sources_from_feed()
-        if self._grad_sources:
-            grads = list(map(self._grad_sources.get, st.param_ids))
-        else:
-            grads = [p.grad for p in params]
-        for g in grads:
-            if g is None:
-                return None
-        dt = st.grad_dtype
-        for g in grads:
-            if g.dtype != dt:
-                return None
-        if not all(map(_is_contiguous, grads)):
-            return None
         # a parameter whose storage was replaced (``p.data = ...``) since the record was made: first and last are
         # looked at here, code that re-homes others calls ``invalidate_tables``
         if (params[0].data_ptr(), params[-1].data_ptr()) != st.param_ptr_ends:
             return None
-        ptrs = list(map(_data_ptr, grads))
-        if ptrs != st.grad_ptrs:
+        if self._grad_sources:
+            found = _addresses(list(map(self._grad_sources.get, st.param_ids)), st.grad_dtype)
+        elif _native is not None:
+            found = self._native_list(gi, params).grad_addresses(st.grad_dtype)
+        else:
+            found = _addresses([p.grad for p in params], st.grad_dtype)
+        if found is None:
+            return None
+        if found != st.grad_ptrs:
+            ptrs = list(memoryview(found).cast("Q"))
             st.table.update_pointers(grads=ptrs, stream=stream_handle(st.device))
-            st.grad_ptrs = ptrs
+            st.grad_ptrs = found
             st.fed_by = None      # a feed's record of what it last pushed into this table is stale from here on
             # the full path's record of what the table points at must not outlive this re-pointing: a later
             # full step with the old addresses would otherwise find them "unchanged" and skip the update
             hit = self._tables.get(st.key)
             if hit is not None and hit[0] is st.table and hit[1] is not None:
                 self._tables[st.key] = (hit[0], (hit[1][0], tuple(ptrs)) + tuple(hit[1][2:]), hit[2])
-        return st, grads
+        return st
 
     def _make_steady(self, gi: int, group, table, grads: List[torch.Tensor], count: Optional[int]) -> None:
         params = group["params"]
@@ -211,7 +229,7 @@ class _FusedBase(torch.optim.Optimizer):
         st.table = table
         st.key = table.cache_key
         st.param_ptr_ends = (params[0].data_ptr(), params[-1].data_ptr())
-        st.grad_ptrs = [g.data_ptr() for g in grads]
+        st.grad_ptrs = _packed(grads)
         st.fed_by = None
         st.grad_dtype = grads[0].dtype
         st.device = params[0].device
@@ -236,10 +254,7 @@ class _FusedBase(torch.optim.Optimizer):
                 for p in params:
                     p.grad = None
                 continue
-            known = self._native_lists.get(gi)
-            if known is None or known[0] is not params or known[1] != len(params):
-                known = self._native_lists[gi] = (params, len(params), _native.TensorList(params))
-            known[2].clear_grads()
+            self._native_list(gi, params).clear_grads()
 
     def _scale_source(self, table: _lib.OptimTable) -> _lib.OptimTable:
         """Tell the table where the gradient scale lives, when that changed since its last launch."""
@@ -263,8 +278,7 @@ class _FusedBase(torch.optim.Optimizer):
                 raise ValueError("model copy must be a contiguous tensor of the master's size and device")
             dtype_code(c.dtype)
             self._model_copies[id(m)] = c
-        self._tables.clear()
-        self._steady.clear()
+        self.invalidate_tables()
 
     def _check_param(self, p: torch.Tensor, g: torch.Tensor) -> None:
         if p.dtype != torch.float32:
@@ -463,11 +477,10 @@ class FusedAdam(_FusedBase):
         if not params:
             return
         clock = self._clocks.get(gi)
-        steady = self._steady_grads(gi, group) if clock is not None else None
-        if steady is not None:
+        st = self._steady_grads(gi, group) if clock is not None else None
+        if st is not None:
             # same parameters, all with usable gradients, as at the step that made the record: the table is in place
             # (re-pointed at the gradients by _steady_grads), only the two launches remain
-            st, _ = steady
             b1, b2 = group["betas"]
             stream = stream_handle(st.device)
             _lib.adam_clock_advance(clock.data_ptr(), group["lr"], b1, b2, self.gate, st.device.index, stream)
@@ -519,9 +532,8 @@ class FusedAdam(_FusedBase):
                 self._capturable_step(gi, group)
             return loss
         for gi, group in enumerate(self.param_groups):
-            steady = self._steady_grads(gi, group)
-            if steady is not None:
-                st, _ = steady
+            st = self._steady_grads(gi, group)
+            if st is not None:
                 st.count += 1
                 st.steps_np += 1.0
                 b1, b2 = group["betas"]
@@ -599,9 +611,8 @@ class FusedSGD(_FusedBase):
             with torch.enable_grad():
                 loss = closure()
         for gi, group in enumerate(self.param_groups):
-            steady = self._steady_grads(gi, group)
-            if steady is not None:
-                st, _ = steady
+            st = self._steady_grads(gi, group)
+            if st is not None:
                 self._scale_source(st.table).sgd_step(group["lr"], group["momentum"], group["dampening"], group["weight_decay"],
                                   group["nesterov"], group["maximize"], first_step=False, grad_scale=self.grad_scale,
                                   gate=self.gate, stream=stream_handle(st.device))
