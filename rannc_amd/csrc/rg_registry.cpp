@@ -21,9 +21,11 @@ using namespace rgbind;
 
 namespace {
 
-// Whether a gradient can be a row of an optimizer table as it is, and its address appended if so.
-bool append_address(const at::Tensor& g, at::ScalarType dtype, std::string& out) {
+// Whether a gradient can be a row of an optimizer table as it is, and its address appended if so.  With an owner it has to be
+// of the owner's size and on its device as well.
+bool append_address(const at::Tensor& g, at::ScalarType dtype, std::string& out, const at::Tensor* owner = nullptr) {
   if (!g.defined() || g.layout() != at::kStrided || g.scalar_type() != dtype || !g.is_contiguous()) return false;
+  if (owner != nullptr && (!owner->defined() || g.numel() != owner->numel() || g.device() != owner->device())) return false;
   const uintptr_t address = reinterpret_cast<uintptr_t>(g.numel() ? g.const_data_ptr() : nullptr);
   out.append(reinterpret_cast<const char*>(&address), sizeof(address));
   return true;
@@ -33,8 +35,23 @@ bool append_address(const at::Tensor& g, at::ScalarType dtype, std::string& out)
 
 class TensorList {
  public:
-  explicit TensorList(const py::object& tensors) : t_(tensor_vector(tensors, "TensorList")) {}
+  explicit TensorList(const py::object& tensors) : t_(tensor_vector(tensors, "TensorList")) {
+    if (!PyList_Check(tensors.ptr()) && !PyTuple_Check(tensors.ptr())) return;
+    objects_.reserve(t_.size());
+    for (const py::handle& o : tensors) objects_.push_back(py::reinterpret_borrow<py::object>(o));
+  }
   explicit TensorList(std::vector<at::Tensor> tensors) : t_(std::move(tensors)) {}
+  // Whether the entries of `tensors` from `first` on are the very objects this list was made of (a list or a tuple); they may be
+  // followed by others.
+  bool holds(const py::sequence& tensors, size_t first) const {
+    const py::object seq = py::reinterpret_steal<py::object>(PySequence_Fast(tensors.ptr(), "holds: not a sequence"));
+    if (!seq) throw py::error_already_set();
+    const size_t n = (size_t)PySequence_Fast_GET_SIZE(seq.ptr());
+    if (objects_.size() != t_.size() || first > n || n - first < objects_.size()) return false;
+    for (size_t i = 0; i < objects_.size(); ++i)
+      if (PySequence_Fast_GET_ITEM(seq.ptr(), (Py_ssize_t)(first + i)) != objects_[i].ptr()) return false;
+    return true;
+  }
   size_t size() const { return t_.size(); }
   const std::vector<at::Tensor>& tensors() const { return t_; }
 
@@ -56,12 +73,22 @@ class TensorList {
     if (views.size() != t_.size()) throw std::invalid_argument("set_grads: the lists differ in length");
     for (size_t i = 0; i < t_.size(); ++i) t_[i].mutable_grad() = views.t_[i];
   }
-  // The addresses of all gradients, one machine word each; None unless every tensor has a contiguous one of `dtype`.
+  // The addresses of all gradients, one machine word each; None unless every tensor has a contiguous one of `dtype`, of its size
+  // and on its device.
   py::object grad_addresses(at::ScalarType dtype) const {
     std::string out;
     out.reserve(t_.size() * sizeof(uintptr_t));
     for (const at::Tensor& t : t_)
-      if (!t.defined() || !append_address(t.grad(), dtype, out)) return py::none();
+      if (!t.defined() || !append_address(t.grad(), dtype, out, &t)) return py::none();
+    return py::bytes(out);
+  }
+  // The same for gradients that are given, one for each tensor.
+  py::object addresses_of(const py::list& grads, at::ScalarType dtype) const {
+    if (grads.size() != t_.size()) return py::none();
+    std::string out;
+    out.reserve(t_.size() * sizeof(uintptr_t));
+    for (size_t i = 0; i < t_.size(); ++i)
+      if (!append_address(tensor_or_undefined(grads[i], "addresses_of"), dtype, out, &t_[i])) return py::none();
     return py::bytes(out);
   }
   void clear_grads() {
@@ -86,6 +113,7 @@ class TensorList {
 
  private:
   std::vector<at::Tensor> t_;
+  std::vector<py::object> objects_;
 };
 
 // ------------------------------------------------------------------------------------------------ GradPlan
@@ -743,7 +771,7 @@ void bind_registry(py::module_& m) {
   });
   m.def("get_amp_master_param", [](long model_param_id) { return global_storage()->get_amp_master_param_tensor(model_param_id); });
 
-  // TensorList.grad_addresses for gradients that are given themselves (None among them: no gradient)
+  // the addresses of gradients without owners to compare them with (None among them: no gradient)
   m.def("tensor_addresses", [](const py::list& tensors, const py::object& dtype) -> py::object {
     const at::ScalarType dt = torch::python::detail::py_object_to_dtype(dtype);
     std::string out;
@@ -766,7 +794,12 @@ void bind_registry(py::module_& m) {
       .def("grads", &TensorList::grads)
       .def("grad_addresses", [](const TensorList& l, const py::object& dtype) {
              return l.grad_addresses(torch::python::detail::py_object_to_dtype(dtype));
-           }, "the gradients' addresses as packed machine words; None unless every tensor has a contiguous gradient of `dtype`")
+           }, "the gradients' addresses as packed machine words; None unless every tensor has a contiguous gradient of `dtype`, of its size and on its device")
+      .def("addresses_of", [](const TensorList& l, const py::list& grads, const py::object& dtype) {
+             return l.addresses_of(grads, torch::python::detail::py_object_to_dtype(dtype));
+           }, "grad_addresses for gradients that are given, one for each tensor (None: it has none)")
+      .def("holds", &TensorList::holds, py::arg("tensors"), py::arg("first") = 0,
+           "whether the entries of `tensors` from `first` on are the very objects this list was made of")
       .def("set_grads", &TensorList::set_grads)
       .def("clear_grads", &TensorList::clear_grads);
 

@@ -12,6 +12,7 @@ them unchanged.  There is no CPU path: parameters must live on the GPU.
 from __future__ import annotations
 
 from array import array
+from operator import is_
 from typing import Dict, List, Optional, Tuple
 
 import torch
@@ -88,8 +89,24 @@ def _own_step(impl):
 class _Steady:
     """What a group's last full step established, for the steps after it: as long as the same parameters all
     have contiguous gradients of the same dtype, a step is one pointer comparison per gradient and one launch."""
-    __slots__ = ("params_obj", "n", "param_ids", "table", "key", "grad_ptrs", "grad_dtype", "steps_buf", "steps_np", "count", "device",
+    __slots__ = ("params", "n", "param_ids", "table", "key", "grad_ptrs", "grad_dtype", "steps_buf", "steps_np", "count", "device",
                  "param_ptr_ends", "fed_by")
+
+    def same(self, params: List[torch.Tensor], first: int = 0) -> bool:
+        """Whether ``params`` holds the record's very parameters from ``first`` on."""
+        if type(self.params) is not tuple:
+            return self.params.holds(params, first)
+        return first + self.n <= len(params) and all(map(is_, self.params, params[first:]))
+
+    def addresses(self, grads: Optional[List[Optional[torch.Tensor]]] = None) -> Optional[bytes]:
+        """Where the gradients lie (those given, or the parameters' own); None unless each parameter has one that the table
+        can read."""
+        if type(self.params) is not tuple:
+            return self.params.grad_addresses(self.grad_dtype) if grads is None else self.params.addresses_of(grads, self.grad_dtype)
+        grads = [p.grad for p in self.params] if grads is None else grads
+        if any(g is not None and (g.numel() != p.numel() or g.device != p.device) for g, p in zip(grads, self.params)):
+            return None
+        return _addresses(grads, self.grad_dtype)
 
 
 class _FusedBase(torch.optim.Optimizer):
@@ -114,7 +131,7 @@ class _FusedBase(torch.optim.Optimizer):
         self._feed = None                          # see set_grad_feed
         self._feed_params: List[torch.Tensor] = []
         self._feed_offsets: Optional[Dict[int, int]] = None
-        self._native_lists: Dict[int, Tuple] = {}  # group index -> (its params list, its length, compiled TensorList)
+        self._native_lists: Dict[int, "_native.TensorList"] = {}     # group index -> its parameters in the compiled module
 
     #: the step can read gradients from tensors other than ``param.grad`` (see ``set_grad_sources``)
     reads_grad_sources = True
@@ -168,22 +185,23 @@ class _FusedBase(torch.optim.Optimizer):
         self._native_lists.clear()
 
     def _native_list(self, gi: int, params):
-        """The compiled module's list of a group's parameters."""
+        """The compiled module's list of a group's parameters: a list may be given other entries in place, so every one is
+        compared (about 1 ns each)."""
         known = self._native_lists.get(gi)
-        if known is None or known[0] is not params or known[1] != len(params):
-            known = self._native_lists[gi] = (params, len(params), _native.TensorList(params))
-        return known[2]
+        if known is None or len(known) != len(params) or not known.holds(params):
+            known = self._native_lists[gi] = _native.TensorList(params)
+        return known
 
     def _steady_grads(self, gi: int, group) -> Optional["_Steady"]:
         """The group's steady-state record, its table pointing at this step's gradients, or None when anything about
         the group differs from the step that made the record (then the full path runs and makes a new one)."""
         st = self._steady.get(gi)
         params = group["params"]
-        if st is None or st.params_obj is not params or len(params) != st.n:
+        if st is None or len(params) != st.n or not st.same(params):
             return None
         if self._feed is not None and not self._grad_sources:
             off = self._feed_offsets.get(gi) if self._feed_offsets is not None else None
-            if (off is not None and self._feed.held() >= off + st.n and dtype_code(st.grad_dtype) == self._feed.source_dtype()
+            if (off is not None and st.same(self._feed_params, off) and self._feed.held() >= off + st.n and dtype_code(st.grad_dtype) == self._feed.source_dtype()
                     and (params[0].data_ptr(), params[-1].data_ptr()) == st.param_ptr_ends):
                 if st.fed_by is not self._feed:
                     self._feed.forget_optim(st.table.handle)      # whatever an earlier table at this address was told
@@ -202,11 +220,9 @@ class _FusedBase(torch.optim.Optimizer):
         if (params[0].data_ptr(), params[-1].data_ptr()) != st.param_ptr_ends:
             return None
         if self._grad_sources:
-            found = _addresses(list(map(self._grad_sources.get, st.param_ids)), st.grad_dtype)
-        elif _native is not None:
-            found = self._native_list(gi, params).grad_addresses(st.grad_dtype)
+            found = st.addresses(list(map(self._grad_sources.get, st.param_ids)))
         else:
-            found = _addresses([p.grad for p in params], st.grad_dtype)
+            found = st.addresses()
         if found is None:
             return None
         if found != st.grad_ptrs:
@@ -224,7 +240,7 @@ class _FusedBase(torch.optim.Optimizer):
     def _make_steady(self, gi: int, group, table, grads: List[torch.Tensor], count: Optional[int]) -> None:
         params = group["params"]
         st = _Steady()
-        st.params_obj, st.n = params, len(params)
+        st.params, st.n = self._native_list(gi, params) if _native is not None else tuple(params), len(params)
         st.param_ids = [id(p) for p in params]
         st.table = table
         st.key = table.cache_key

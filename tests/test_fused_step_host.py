@@ -1,0 +1,208 @@
+"""The host side of the fused optimizers' steps without a GPU: which parameters, gradients and counts reach a table, with the
+tables replaced by a record of what they are told.  Each test runs with the compiled module and without it."""
+import pytest
+import torch
+
+from rannc_amd import fused_optim
+from rannc_amd.fused_optim import FusedAdam, FusedAdamW, FusedSGD
+
+
+class Param(torch.nn.Parameter):
+    """A CPU parameter that passes for one on the GPU."""
+    is_cuda = True
+
+
+class Table:
+    """What ``_lib.OptimTable`` is told."""
+    made = []
+    refuse = None          # an exception that the next launches raise
+
+    def __init__(self, device, params, grads, state1, state2, copies, numels, grad_dtypes, copy_dtypes=None, scales1=None, scales2=None):
+        self.params, self.grads, self.state1, self.state2 = list(params), list(grads), state1, state2
+        self.numels, self.grad_dtypes, self.steps = list(numels), grad_dtypes, []
+        self.handle = id(self)
+        Table.made.append(self)
+
+    def update_pointers(self, params=None, grads=None, state1=None, state2=None, copies=None, stream=0):
+        for name, given in (("params", params), ("grads", grads), ("state1", state1), ("state2", state2)):
+            if given is not None:
+                setattr(self, name, list(given))
+
+    def adam_step(self, lr, beta1, beta2, eps, weight_decay, step, **kw):
+        if Table.refuse is not None:
+            raise Table.refuse
+        self.steps.append((step, list(self.params), list(self.grads)))
+
+    def sgd_step(self, *args, first_step=False, **kw):
+        if Table.refuse is not None:
+            raise Table.refuse
+        self.steps.append((first_step, list(self.params), list(self.grads)))
+
+
+@pytest.fixture(params=["compiled", "python"], autouse=True)
+def route(request, monkeypatch):
+    if request.param == "python":
+        monkeypatch.setattr(fused_optim, "_native", None)
+    elif fused_optim._native is None:
+        pytest.skip("the compiled module is not built")
+    monkeypatch.setattr(fused_optim._lib, "OptimTable", Table)
+    monkeypatch.setattr(fused_optim, "stream_handle", lambda device: 0)
+    monkeypatch.setattr(Table, "made", [])
+    monkeypatch.setattr(Table, "refuse", None)
+    return request.param
+
+
+MAKE = {"adam": lambda ps: FusedAdam(ps, lr=1e-2), "adamw8": lambda ps: FusedAdamW(ps, lr=1e-2, state_bits=8),
+        "sgd": lambda ps: FusedSGD(ps, lr=0.05)}
+
+
+@pytest.fixture(params=sorted(MAKE))
+def make(request):
+    return MAKE[request.param]
+
+
+def parameters(sizes=(4, 6, 5)):
+    return [Param(torch.zeros(n)) for n in sizes]
+
+
+def give(params):
+    for p in params:
+        p.grad = torch.ones_like(p.detach())
+
+
+# ---------------------------------------------------------------- entries of a group replaced in place
+
+@pytest.mark.parametrize("place", [0, 1, 2])
+@pytest.mark.parametrize("size", [4, 400000])
+def test_replaced_parameters_bring_their_own_gradients(make, place, size):
+    ps = parameters()
+    opt = make(ps)
+    for _ in range(3):
+        give(ps)
+        opt.step()
+    group = opt.param_groups[0]["params"]
+    old, new = group[place], Param(torch.zeros(size))
+    group[place] = new
+    if not isinstance(opt, FusedSGD):         # the count moves along, so that the group stays in step
+        opt.state[new]["step"] = torch.tensor(float(opt.state[old]["step"]))
+        opt._make_moments(0, [new])
+    kept = old.grad                            # nothing clears it: it is no longer the optimizer's
+    for _ in range(3):
+        for p in group:
+            p.grad = torch.ones_like(p.detach())
+        opt.step()
+        table = Table.made[-1]
+        _, params, grads = table.steps[-1]
+        assert params == [p.data_ptr() for p in group] and grads == [p.grad.data_ptr() for p in group]
+        assert table.numels == [p.numel() for p in group] and kept.data_ptr() not in grads
+
+
+def test_cleared_gradients_are_those_of_the_moment(make):
+    ps = parameters()
+    opt = make(ps)
+    give(ps)
+    opt.zero_grad()
+    new = Param(torch.zeros(7))
+    old, opt.param_groups[0]["params"][1] = ps[1], new
+    give([old, new])
+    opt.zero_grad()
+    assert new.grad is None and old.grad is not None
+
+
+def test_steps_stay_on_the_short_path(make, monkeypatch):
+    """An unchanged group, also one whose list was replaced by an equal one, is not looked at parameter by parameter."""
+    ps = parameters()
+    opt = make(ps)
+    for _ in range(2):
+        give(ps)
+        opt.step()
+    monkeypatch.setattr(opt, "_table", None)
+    for _ in range(2):
+        give(ps)
+        opt.step()
+    opt.param_groups[0]["params"] = list(ps)
+    give(ps)
+    opt.step()
+    assert len(Table.made) == 1 and len(Table.made[0].steps) == 5
+
+
+@pytest.mark.parametrize("sources", [False, True])
+def test_gradients_of_another_size_are_refused(make, sources):
+    """A steady group whose parameter (and gradient source) changed size behind the optimizer's back."""
+    ps = parameters()
+    opt = make(ps)
+    for _ in range(2):
+        give(ps)
+        opt.step()
+    before = len(Table.made[0].steps)
+    short = torch.ones(2)
+    if sources:
+        opt.set_grad_sources(ps, [ps[0].grad, short, ps[2].grad])
+    else:
+        class Short(Param):
+            grad = short
+        ps[1].__class__ = Short
+        if fused_optim._native is not None:
+            pytest.skip("the compiled module reads the real gradient, whose size torch checks")
+    with pytest.raises(ValueError, match="size"):
+        opt.step()
+    assert len(Table.made[0].steps) == before
+
+
+def test_feed_rows_have_to_be_the_groups_parameters(make):
+    """A feed whose parameters have the group's ends but another one between them is not pushed into the group's table."""
+    if fused_optim._native is None:
+        pytest.skip("only the compiled module has feeds")
+    ps = parameters()
+    opt = make(ps)
+    for _ in range(2):
+        give(ps)
+        opt.step()
+
+    class Feed:
+        pushed = 0
+
+        def held(self):
+            return 3
+
+        def source_dtype(self):
+            return fused_optim._lib.RG_F32
+
+        def sources(self):
+            return self.grads
+
+        def forget_optim(self, handle):
+            pass
+
+        def push_sources_to_optim(self, handle, off, n):
+            Feed.pushed += 1
+            return True
+
+    feed = Feed()
+    other = Param(torch.zeros(6))
+    feed.grads = [torch.ones_like(p.detach()) for p in ps]
+    opt.set_grad_feed(feed, [ps[0], other, ps[2]])
+    opt.step()
+    assert Feed.pushed == 0 and Table.made[-1].steps[-1][2] == [feed.grads[0].data_ptr(), ps[1].grad.data_ptr(), feed.grads[2].data_ptr()]
+    opt.set_grad_feed(feed, list(ps))
+    opt.step()
+    assert Feed.pushed == 1
+
+
+def test_lists_know_their_objects():
+    native = fused_optim._native
+    if native is None:
+        pytest.skip("the compiled module is switched off")
+    ps = parameters()
+    held = native.TensorList(ps)
+    assert held.holds(ps) and held.holds(tuple(ps)) and held.holds([None] + ps + [None], 1) and not held.holds(ps, 1)
+    assert not held.holds(ps[:2]) and not held.holds(ps[::-1]) and not held.holds(ps, 7) and not held.holds([])
+    alias = ps[1].detach()                     # the same memory, another object
+    assert not held.holds([ps[0], alias, ps[2]])
+    assert native.TensorList([]).holds([])
+    give(ps)
+    grads = [p.grad for p in ps]
+    assert held.addresses_of(grads, torch.float32) == held.grad_addresses(torch.float32)
+    for bad in (grads[:2], [grads[0], None, grads[2]], [grads[0], torch.ones(5), grads[2]], [g.half() for g in grads],
+                [grads[0], grads[1].to("meta"), grads[2]]):
+        assert held.addresses_of(bad, torch.float32) is None
