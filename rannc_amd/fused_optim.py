@@ -305,6 +305,7 @@ class _FusedBase(torch.optim.Optimizer):
             raise ValueError("sparse gradients are not supported")
         if not g.is_contiguous() or g.device != p.device or g.numel() != p.numel():
             raise ValueError("gradient must be contiguous, on the parameter's device and of its size")
+        dtype_code(g.dtype)
 
     def _table(self, key: Tuple, params: List[torch.Tensor], grads: List[torch.Tensor],
                state1: Optional[List[torch.Tensor]], state2: Optional[List[torch.Tensor]],
@@ -381,25 +382,30 @@ class FusedAdam(_FusedBase):
         self._buffers8: Dict[int, List[Dict[str, torch.Tensor]]] = {}      # group index -> the buffers its 8-bit states lie in
 
     def _make_moments(self, gi: int, params: List[torch.Tensor], loaded: Optional[List[Dict]] = None) -> None:
-        """Moments for ``params`` of one group (``step`` is the caller's): zeros, or in 8 bits what ``loaded`` holds in 32."""
-        if self.state_bits == 32:
-            for p in params:
-                self.state[p]["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-                self.state[p]["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-            return
+        """Moments for ``params`` of one group: zeros (with a count of zero where there is none), or in 8 bits what ``loaded``
+        holds in 32.  All of them or, when something raises, none."""
         if not params:
             return
+        if self.state_bits == 32:
+            made = [{name: torch.zeros_like(p, memory_format=torch.preserve_format) for name in ("exp_avg", "exp_avg_sq")}
+                    for p in params]
+            self._add_state(params, made)
+            return
         buffers: Dict[str, torch.Tensor] = {}
-        made: List[Dict[str, torch.Tensor]] = [{} for _ in params]
+        made = [{} for _ in params]
         for name in ("exp_avg", "exp_avg_sq"):
             codes, scales, buffers[name], buffers[name + "_scale"] = allocate_state8(params)
             for entry, c, s in zip(made, codes, scales):
                 entry[name], entry[name + "_scale"] = c, s
         if loaded is not None:
             self._convert_moments(made, loaded, to_codes=True)
-        for p, entry in zip(params, made):       # only now: whatever failed before has left the states as they were
-            self.state[p].update(entry)
+        self._add_state(params, made)
         self._buffers8.setdefault(gi, []).append(buffers)
+
+    def _add_state(self, params: List[torch.Tensor], made: List[Dict[str, torch.Tensor]]) -> None:
+        steps = [self.state[p]["step"] if "step" in self.state.get(p, {}) else torch.tensor(0.0, dtype=torch.float32) for p in params]
+        for p, step, entry in zip(params, steps, made):
+            self.state[p].update(step=step, **entry)
 
     def _moments(self, params: List[torch.Tensor]):
         """The state columns ``_table`` takes for these parameters."""
@@ -550,49 +556,44 @@ class FusedAdam(_FusedBase):
         for gi, group in enumerate(self.param_groups):
             st = self._steady_grads(gi, group)
             if st is not None:
-                st.count += 1
-                st.steps_np += 1.0
                 b1, b2 = group["betas"]
-                self._scale_source(st.table).adam_step(group["lr"], b1, b2, group["eps"], group["weight_decay"], st.count,
+                self._scale_source(st.table).adam_step(group["lr"], b1, b2, group["eps"], group["weight_decay"], st.count + 1,
                                    decoupled=self._decoupled, maximize=group["maximize"], grad_scale=self.grad_scale,
                                    gate=self.gate, stream=stream_handle(st.device))
+                st.count += 1                    # behind the launch: a step that is refused does not count
+                st.steps_np += 1.0
                 continue
             self._steady.pop(gi, None)
             by_step: Dict[int, List[torch.Tensor]] = {}
-            step_tensors = []
             grad_of: Dict[int, torch.Tensor] = {}
-            fresh = []
             found = []
-            for p in group["params"]:            # all of them are looked at before any count moves
+            for p in group["params"]:            # everything that can be refused or fail comes before the first launch,
                 g = self._grad_of(p)
                 if g is None:
                     continue
                 self._check_param(p, g)
                 found.append(p)
                 grad_of[id(p)] = g
+            self._make_moments(gi, [p for p in found if "exp_avg" not in self.state.get(p, {})])
+            self._settle_moments(gi, group["params"])
             for p in found:
-                st = self.state[p]
-                if "exp_avg" not in st:
-                    st.setdefault("step", torch.tensor(0.0, dtype=torch.float32))
-                    fresh.append(p)
                 # ``step`` stays a tensor (torch.optim's state layout); its integer value is mirrored
                 # here so that a step costs one batched increment instead of one tensor op per parameter
-                t = st["step"]
+                t = self.state[p]["step"]
+                if not torch.is_tensor(t):
+                    t = self.state[p]["step"] = torch.tensor(float(t), dtype=torch.float32)
                 seen = self._steps.get(id(p))
-                count = (seen[1] if seen is not None and seen[0] is t else int(t)) + 1
-                self._steps[id(p)] = (t, count)
-                step_tensors.append(t)
-                by_step.setdefault(count, []).append(p)
-            self._make_moments(gi, fresh)
-            self._settle_moments(gi, group["params"])
-            if step_tensors:
-                torch._foreach_add_(step_tensors, 1)
-            for step, ps in by_step.items():
-                table = self._table((gi, tuple(id(p) for p in ps)), ps, [grad_of[id(p)] for p in ps], *self._moments(ps))
+                by_step.setdefault((seen[1] if seen is not None and seen[0] is t else int(t)) + 1, []).append(p)
+            tables = [self._table((gi, tuple(id(p) for p in ps)), ps, [grad_of[id(p)] for p in ps], *self._moments(ps))
+                      for ps in by_step.values()]
+            for table, (step, ps) in zip(tables, by_step.items()):
                 b1, b2 = group["betas"]
                 self._scale_source(table).adam_step(group["lr"], b1, b2, group["eps"], group["weight_decay"], step,
                                 decoupled=self._decoupled, maximize=group["maximize"], grad_scale=self.grad_scale,
                                 gate=self.gate, stream=stream_handle(ps[0].device))
+                counts = [self.state[p]["step"] for p in ps]          # ... and the counts move behind it
+                torch._foreach_add_(counts, 1)
+                self._steps.update((id(p), (t, step)) for p, t in zip(ps, counts))
                 if len(by_step) == 1 and len(ps) == len(group["params"]):
                     self._make_steady(gi, group, table, [grad_of[id(p)] for p in ps], step)
         return loss

@@ -206,3 +206,77 @@ def test_lists_know_their_objects():
     for bad in (grads[:2], [grads[0], None, grads[2]], [grads[0], torch.ones(5), grads[2]], [g.half() for g in grads],
                 [grads[0], grads[1].to("meta"), grads[2]]):
         assert held.addresses_of(bad, torch.float32) is None
+
+
+# ---------------------------------------------------------------- steps that are refused or fail
+
+def _raise(error):
+    def anything(*args, **kwargs):
+        raise error
+    return anything
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("earlier", [0, 1, 2])          # steps before: none, one (the next is a full one), two (a steady one)
+@pytest.mark.parametrize("what", ["gradient type", "moments", "conversion", "table", "launch"])
+def test_failed_steps_count_for_nothing(bits, earlier, what, monkeypatch):
+    ps = parameters()
+    opt = FusedAdam(ps, state_bits=bits)
+    for _ in range(earlier):
+        give(ps)
+        opt.step()
+    if earlier == 1:
+        opt.invalidate_tables()
+    give(ps)
+    for _ in range(3):
+        with monkeypatch.context() as m:
+            if what == "gradient type":
+                opt.set_grad_sources(ps, [p.grad.double() if i == 1 else p.grad for i, p in enumerate(ps)])
+            elif what == "moments":
+                if earlier:
+                    pytest.skip("they are there")
+                made = torch.zeros if bits == 8 else torch.zeros_like          # the second allocation fails
+                calls = []
+                m.setattr(torch, made.__name__, lambda *a, **k: made(*a, **k) if not calls.append(1) and len(calls) % 2 else _raise(MemoryError("none left"))())
+            elif what == "conversion":
+                opt.invalidate_tables()
+                m.setattr(FusedAdam, "_settle_moments", _raise(MemoryError("none left")))
+            elif what == "table":
+                opt.invalidate_tables()
+                m.setattr(fused_optim._lib, "OptimTable", _raise(MemoryError("none left")))
+            else:
+                m.setattr(Table, "refuse", ValueError("bad hyper-parameters"))
+            with pytest.raises((MemoryError, ValueError, TypeError)):
+                opt.step()
+        opt.set_grad_sources([], [])
+        assert sum(len(t.steps) for t in Table.made) == earlier
+        for p in ps:
+            state = opt.state.get(p, {})
+            assert float(state.get("step", 0)) == earlier and ("exp_avg" in state) == ("exp_avg_sq" in state)
+            assert what != "moments" or not state
+    for step in range(earlier + 1, earlier + 4):
+        give(ps)
+        opt.step()
+        assert Table.made[-1].steps[-1][0] == step and all(float(opt.state[p]["step"]) == step for p in ps)
+
+
+def test_counts_of_parameters_that_join_late():
+    ps = parameters()
+    opt = FusedAdam(ps)
+    for step in range(1, 6):
+        give(ps if step > 2 else ps[:2])
+        opt.step()
+        assert [float(opt.state[p]["step"]) for p in ps[:2]] == [step] * 2
+        assert step <= 2 or float(opt.state[ps[2]]["step"]) == step - 2
+    counts = [s[0] for t in Table.made for s in t.steps]
+    assert sorted(counts) == [1, 1, 2, 2, 3, 3, 4, 5]
+
+
+def test_counts_given_as_numbers():
+    ps = parameters()
+    opt = FusedAdam(ps)
+    for p in ps:
+        opt.state[p].update(step=4, exp_avg=torch.zeros_like(p), exp_avg_sq=torch.zeros_like(p))
+    give(ps)
+    opt.step()
+    assert Table.made[-1].steps[-1][0] == 5 and all(float(opt.state[p]["step"]) == 5 for p in ps)
