@@ -636,6 +636,7 @@ class FusedSGD(_FusedBase):
                 continue
             self._steady.pop(gi, None)
             fresh, seasoned = [], []
+            made: Dict[int, torch.Tensor] = {}
             grad_of: Dict[int, torch.Tensor] = {}
             for p in group["params"]:
                 g = self._grad_of(p)
@@ -643,22 +644,28 @@ class FusedSGD(_FusedBase):
                     continue
                 self._check_param(p, g)
                 grad_of[id(p)] = g
-                st = self.state[p]
-                if group["momentum"] != 0 and st.get("momentum_buffer") is None:
+                if group["momentum"] != 0 and self.state.get(p, {}).get("momentum_buffer") is None:
                     # zeros, not empty: if the first launch is gated off on the device the buffer must
                     # not reach the next step with whatever the memory held
-                    st["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                    made[id(p)] = torch.zeros_like(p, memory_format=torch.preserve_format)
                     fresh.append(p)
                 else:
                     seasoned.append(p)
+            tables = []                          # all of them before the first launch: what fails leaves the state as it was
             for first, ps in ((True, fresh), (False, seasoned)):
                 if not ps:
                     continue
-                bufs = [self.state[p]["momentum_buffer"] for p in ps] if group["momentum"] != 0 else None
-                table = self._table((gi, first, tuple(id(p) for p in ps)), ps, [grad_of[id(p)] for p in ps], bufs, None)
+                bufs = None
+                if group["momentum"] != 0:
+                    bufs = [made[id(p)] if first else self.state[p]["momentum_buffer"] for p in ps]
+                tables.append((first, ps, self._table((gi, first, tuple(id(p) for p in ps)), ps, [grad_of[id(p)] for p in ps], bufs, None)))
+            for first, ps, table in tables:
                 self._scale_source(table).sgd_step(group["lr"], group["momentum"], group["dampening"], group["weight_decay"],
                                group["nesterov"], group["maximize"], first_step=first, grad_scale=self.grad_scale,
                                gate=self.gate, stream=stream_handle(ps[0].device))
+                if first and made:               # a buffer is the state's once its first step has been launched
+                    for p in ps:
+                        self.state[p]["momentum_buffer"] = made[id(p)]
                 if not first and not fresh and len(ps) == len(group["params"]):
                     self._make_steady(gi, group, table, [grad_of[id(p)] for p in ps], None)
         return loss

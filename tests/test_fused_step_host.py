@@ -280,3 +280,31 @@ def test_counts_given_as_numbers():
     give(ps)
     opt.step()
     assert Table.made[-1].steps[-1][0] == 5 and all(float(opt.state[p]["step"]) == 5 for p in ps)
+
+
+@pytest.mark.parametrize("what", ["gradient type", "buffers", "table", "launch"])
+def test_failed_first_step_leaves_no_momentum(what, monkeypatch):
+    """Momentum starts as the gradient itself, not dampened: a first step that failed is still to come."""
+    ps = parameters()
+    opt = FusedSGD(ps, lr=0.1, momentum=0.9, dampening=0.5)
+    give(ps)
+    for _ in range(2):
+        with monkeypatch.context() as m:
+            if what == "gradient type":
+                opt.set_grad_sources(ps, [p.grad.double() if i == 1 else p.grad for i, p in enumerate(ps)])
+            elif what == "buffers":
+                made, calls = torch.zeros_like, []
+                m.setattr(torch, "zeros_like", lambda *a, **k: made(*a, **k) if not calls.append(1) and len(calls) < 2 else _raise(MemoryError("none left"))())
+            elif what == "table":
+                m.setattr(fused_optim._lib, "OptimTable", _raise(MemoryError("none left")))
+            else:
+                m.setattr(Table, "refuse", ValueError("bad hyper-parameters"))
+            with pytest.raises((MemoryError, ValueError, TypeError)):
+                opt.step()
+        opt.set_grad_sources([], [])
+        assert not any("momentum_buffer" in opt.state.get(p, {}) for p in ps)
+    for first in (True, False, False):
+        give(ps)
+        opt.step()
+        assert Table.made[-1].steps[-1][0] is first and len(Table.made[-1].steps[-1][1]) == 3
+        assert list(Table.made[-1].state1) == [opt.state[p]["momentum_buffer"].data_ptr() for p in ps]
