@@ -307,13 +307,31 @@ class _FusedBase(torch.optim.Optimizer):
             raise ValueError("gradient must be contiguous, on the parameter's device and of its size")
         dtype_code(g.dtype)
 
+    @staticmethod
+    def _check_rows(params, copies, state1, state2, scales) -> None:
+        """What a table is pointed at beside the gradients has to fit the parameters as they are now: a table knows addresses
+        and the parameters' sizes only."""
+        dtype = torch.float32 if scales is None else torch.float8_e4m3fn
+        for i, p in enumerate(params):
+            if p.device != params[0].device:
+                raise ValueError("the parameters of a group must be on one device")
+            held = [(column[i], dtype, p.numel()) for column in (state1, state2) if column is not None]
+            if scales is not None:
+                held += [(column[i], torch.float32, _lib.state8_num_scales(p.numel())) for column in scales]
+            if copies[i] is not None:
+                held.append((copies[i], copies[i].dtype, p.numel()))
+            for t, want, numel in held:
+                if t.dtype != want or t.numel() != numel or t.device != p.device or not t.is_contiguous():
+                    raise ValueError(f"parameter {i} has {p.numel()} elements on {p.device}; of its state or model copy, a tensor has "
+                                     f"{t.numel()} elements, {t.dtype}, on {t.device}{'' if t.is_contiguous() else ', not contiguous'}")
+
     def _table(self, key: Tuple, params: List[torch.Tensor], grads: List[torch.Tensor],
                state1: Optional[List[torch.Tensor]], state2: Optional[List[torch.Tensor]],
                scales: Optional[Tuple[List[torch.Tensor], List[torch.Tensor]]] = None) -> _lib.OptimTable:
         """Table for this exact list of parameters and gradient dtypes, re-pointed when any address moved.  ``scales``:
         the states are in 8 bits, and these are their blocks' scales."""
         copies = [self._model_copies.get(id(p)) for p in params]
-        key = key + (tuple(g.dtype for g in grads),)
+        key = key + (tuple(g.dtype for g in grads), tuple(p.numel() for p in params))      # what a table cannot change
         ptrs = (tuple(p.data_ptr() for p in params), tuple(g.data_ptr() for g in grads),
                 tuple(s.data_ptr() for s in state1) if state1 is not None else None,
                 tuple(s.data_ptr() for s in state2) if state2 is not None else None,
@@ -324,6 +342,8 @@ class _FusedBase(torch.optim.Optimizer):
         dev = params[0].device
         if hit is not None and scales is not None and hit[2][4] != (ptrs[2], ptrs[3]) + scale_ptrs:
             hit = None          # 8-bit states have moved, which a table cannot follow: make another
+        if hit is None or hit[1] != ptrs:
+            self._check_rows(params, copies, state1, state2, scales)
         if hit is None:
             table = _lib.OptimTable(dev.index, ptrs[0], ptrs[1], ptrs[2], ptrs[3],
                                     ptrs[4] if any(ptrs[4]) else None, [p.numel() for p in params],

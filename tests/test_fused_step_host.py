@@ -308,3 +308,51 @@ def test_failed_first_step_leaves_no_momentum(what, monkeypatch):
         opt.step()
         assert Table.made[-1].steps[-1][0] is first and len(Table.made[-1].steps[-1][1]) == 3
         assert list(Table.made[-1].state1) == [opt.state[p]["momentum_buffer"].data_ptr() for p in ps]
+
+
+# ---------------------------------------------------------------- parameters whose memory changes
+
+@pytest.mark.parametrize("size", [3, 4, 500])
+def test_parameters_of_another_size_get_a_table_of_their_own(size):
+    """``p.data`` replaced between steps: a table keeps the sizes that it was made with."""
+    ps = parameters()
+    opt = FusedSGD(ps, lr=0.1)
+    for _ in range(2):
+        give(ps)
+        opt.step()
+    ps[0].grad = None
+    ps[0].data = torch.zeros(size)
+    give(ps)
+    opt.step()
+    assert Table.made[-1].numels == [size, 6, 5] and Table.made[-1].steps[-1][1] == [p.data_ptr() for p in ps]
+    assert len(Table.made) == (1 if size == 4 else 2)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("size", [3, 500])
+def test_states_of_another_size_are_refused(bits, size):
+    ps = parameters()
+    opt = FusedAdam(ps, state_bits=bits)
+    for _ in range(2):
+        give(ps)
+        opt.step()
+    ps[0].grad = None
+    ps[0].data = torch.zeros(size)
+    give(ps)
+    with pytest.raises(ValueError, match="elements"):
+        opt.step()
+    assert sum(len(t.steps) for t in Table.made) == 2 and float(opt.state[ps[0]]["step"]) == 2
+
+
+@pytest.mark.parametrize("name,wrong", [("exp_avg", lambda t: t.double()), ("exp_avg", lambda t: t[:3]), ("exp_avg_sq", lambda t: t.to("meta")),
+                                        ("exp_avg_sq", lambda t: t.repeat_interleave(2)[::2])])
+def test_states_that_do_not_fit_are_refused(name, wrong):
+    ps = parameters()
+    opt = FusedAdam(ps)
+    give(ps)
+    opt.step()
+    opt.state[ps[0]][name] = wrong(opt.state[ps[0]][name])
+    opt.invalidate_tables()
+    with pytest.raises(ValueError, match="elements"):
+        opt.step()
+    assert float(opt.state[ps[0]]["step"]) == 1
