@@ -172,6 +172,10 @@ class _FusedBase(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict) -> None:
         super().load_state_dict(state_dict)
+        for st in self.state.values():          # a checkpoint may hold moments in another memory order (channels last)
+            for name, value in st.items():
+                if torch.is_tensor(value) and value.layout == torch.strided and not value.is_contiguous():
+                    st[name] = value.contiguous()
         self._steady.clear()          # the state tensors are new objects: the next step rebuilds tables and counters
         self._tables.clear()
         self._steps.clear()

@@ -356,3 +356,24 @@ def test_states_that_do_not_fit_are_refused(name, wrong):
     with pytest.raises(ValueError, match="elements"):
         opt.step()
     assert float(opt.state[ps[0]]["step"]) == 1
+
+
+@pytest.mark.parametrize("make", [lambda ps: FusedAdam(ps), lambda ps: FusedSGD(ps, momentum=0.9)], ids=["adam", "sgd"])
+def test_loaded_states_in_another_memory_order(make):
+    ps = [Param(torch.zeros(2, 3, 4, 5))]
+    opt = make(ps)
+    for _ in range(2):
+        give(ps)
+        opt.step()
+    sd = opt.state_dict()
+    want = {}
+    for name, value in sd["state"][0].items():
+        if torch.is_tensor(value) and value.dim() == 4:
+            want[name] = torch.arange(120.0).view(2, 3, 4, 5)
+            sd["state"][0][name] = want[name].to(memory_format=torch.channels_last)
+    assert want
+    opt.load_state_dict(sd)
+    for name, value in want.items():
+        assert opt.state[ps[0]][name].is_contiguous() and torch.equal(opt.state[ps[0]][name], value)
+    opt.step()
+    assert list(Table.made[-1].state1) == [opt.state[ps[0]][list(want)[0]].data_ptr()]
