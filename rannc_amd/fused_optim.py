@@ -522,6 +522,9 @@ class FusedAdam(_FusedBase):
         params = group["params"]
         if not params:
             return
+        # the clock's kernel would have counted the step by the time the update is refused for these
+        if not (group["eps"] >= 0 and group["weight_decay"] >= 0):
+            raise ValueError(f"invalid Adam hyper-parameters: eps {group['eps']}, weight_decay {group['weight_decay']}")
         clock = self._clocks.get(gi)
         st = self._steady_grads(gi, group) if clock is not None else None
         if st is not None:
@@ -540,16 +543,19 @@ class FusedAdam(_FusedBase):
         if any(g is None for g in grads):
             raise RuntimeError("a capturable optimizer needs a gradient for every parameter at every step")
         dev = params[0].device
+        for p, g in zip(params, grads):
+            self._check_param(p, g)
+        fresh = [p for p in params if "exp_avg" not in self.state.get(p, {})]
         if clock is None:
-            counts = set()
-            for p, g in zip(params, grads):
-                self._check_param(p, g)
-            fresh = [p for p in params if "exp_avg" not in self.state[p]]
-            counts.update(int(self.state[p]["step"]) if "exp_avg" in self.state[p] else 0 for p in params)
-            self._make_moments(gi, fresh)
-            self._settle_moments(gi, params)
+            counts = {0 if "exp_avg" not in self.state.get(p, {}) else int(self.state[p]["step"]) for p in params}
             if len(counts) != 1:
                 raise RuntimeError("a capturable optimizer keeps one step count per group; the loaded counts differ")
+        elif fresh:
+            raise RuntimeError("a capturable optimizer keeps one step count per group: a parameter without moments joined it")
+        self._make_moments(gi, fresh)
+        self._settle_moments(gi, params)
+        table = self._table((gi, "capturable", tuple(id(p) for p in params)), list(params), grads, *self._moments(params))
+        if clock is None:
             clock = torch.zeros(_lib.ADAM_CLOCK_BYTES // 4, dtype=torch.float32, device=dev)
             count = counts.pop()
             if count:
@@ -558,7 +564,6 @@ class FusedAdam(_FusedBase):
             for p in params:
                 self.state[p]["step"] = clock[4]          # every parameter's count is the group's, on the device
             self._clocks[gi] = clock
-        table = self._table((gi, "capturable"), params, grads, *self._moments(params))
         b1, b2 = group["betas"]
         stream = stream_handle(dev)
         _lib.adam_clock_advance(clock.data_ptr(), group["lr"], b1, b2, self.gate, dev.index, stream)

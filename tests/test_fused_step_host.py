@@ -377,3 +377,83 @@ def test_loaded_states_in_another_memory_order(make):
         assert opt.state[ps[0]][name].is_contiguous() and torch.equal(opt.state[ps[0]][name], value)
     opt.step()
     assert list(Table.made[-1].state1) == [opt.state[ps[0]][list(want)[0]].data_ptr()]
+
+
+# ---------------------------------------------------------------- the step count on the device
+
+@pytest.fixture
+def clock(monkeypatch):
+    """Counts what the clock's kernel and the step that reads it are told."""
+    ticks = []
+    monkeypatch.setattr(fused_optim._lib, "adam_clock_advance", lambda *args: ticks.append(args))
+
+    def adam_step_clocked(self, clock_ptr, lr, beta1, beta2, eps, weight_decay, **kw):
+        if not (eps >= 0 and weight_decay >= 0):
+            raise ValueError("bad hyper-parameters")
+        self.steps.append((len(ticks), list(self.params), list(self.grads)))
+    monkeypatch.setattr(Table, "adam_step_clocked", adam_step_clocked, raising=False)
+    return ticks
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("bad", [dict(eps=-1.0), dict(weight_decay=-0.1), dict(eps=float("nan"))])
+def test_refused_capturable_step_does_not_advance_the_clock(clock, bits, bad):
+    ps = parameters()
+    opt = FusedAdam(ps, capturable=True, state_bits=bits)
+    give(ps)
+    group = opt.param_groups[0]
+    good = {k: group[k] for k in bad}
+    for steps in (0, 1, 2):                         # before the first step, and before a steady one
+        group.update(bad)
+        with pytest.raises(ValueError, match="hyper-parameters"):
+            opt.step()
+        assert len(clock) == steps
+        group.update(good)
+        opt.step()
+
+
+@pytest.mark.parametrize("bad,match", [(lambda g: g.repeat_interleave(2)[::2], "contiguous"), (lambda g: g[:1].expand(6), "contiguous"),
+                                       (lambda g: g[:5], "size"), (lambda g: g.double(), "dtype")])
+def test_capturable_steps_check_gradients_every_time(clock, bad, match):
+    ps = parameters()
+    opt = FusedAdam(ps, capturable=True)
+    for _ in range(3):
+        give(ps)
+        opt.step()
+    opt.set_grad_sources(ps, [bad(p.grad) if i == 1 else p.grad for i, p in enumerate(ps)])
+    with pytest.raises(ValueError, match=match):
+        opt.step()
+    assert len(clock) == 3
+    opt.set_grad_sources([], [])
+    opt.step()
+    assert len(clock) == 4 and Table.made[-1].steps[-1][0] == 4
+
+
+@pytest.mark.parametrize("size", [3, 6, 500])
+def test_capturable_group_with_another_parameter(clock, size):
+    ps = parameters()
+    opt = FusedAdam(ps, capturable=True)
+    for _ in range(2):
+        give(ps)
+        opt.step()
+    group = opt.param_groups[0]["params"]
+    old, new = group[1], Param(torch.zeros(size))
+    group[1] = new
+    new.grad = torch.ones(size)
+    with pytest.raises(RuntimeError, match="without moments"):
+        opt.step()
+    opt.state[new] = {"step": opt.state[old]["step"], "exp_avg": torch.zeros(size), "exp_avg_sq": torch.zeros(size)}
+    opt.step()
+    assert Table.made[-1].numels == [4, size, 5] and Table.made[-1].steps[-1][1] == [p.data_ptr() for p in group]
+    assert Table.made[0].numels == [4, 6, 5]
+
+
+def test_differing_counts_leave_the_state_alone(clock):
+    ps = parameters()
+    opt = FusedAdam(ps, capturable=True)
+    opt.state[ps[0]] = {"step": torch.tensor(3.0), "exp_avg": torch.zeros(4), "exp_avg_sq": torch.zeros(4)}
+    give(ps)
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="counts differ"):
+            opt.step()
+        assert list(opt.state) == [ps[0]] and not Table.made
