@@ -402,6 +402,8 @@ class FusedAdam(_FusedBase):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, maximize=maximize))
         self.capturable = bool(capturable)
         self.state_bits = int(state_bits)
+        if self.state_bits == 8:
+            self._conversion_hook = super().register_state_dict_post_hook(FusedAdam._give_moments)
         self._clocks: Dict[int, torch.Tensor] = {}       # group index -> its rg_adam_clock (8 float32 words on the device)
         self._buffers8: Dict[int, List[Dict[str, torch.Tensor]]] = {}      # group index -> the buffers its 8-bit states lie in
 
@@ -470,10 +472,14 @@ class FusedAdam(_FusedBase):
                 plan.dequantize()
             plan.close()
 
-    def state_dict(self) -> Dict:
-        packed = super().state_dict()
-        if self.state_bits == 32:
-            return packed
+    def register_state_dict_post_hook(self, hook, prepend: bool = False):
+        handle = super().register_state_dict_post_hook(hook, prepend)
+        if self.state_bits == 8:        # the conversion stays the first of them: hooks see float32 moments
+            self._optimizer_state_dict_post_hooks.move_to_end(self._conversion_hook.id, last=False)
+        return handle
+
+    def _give_moments(self, packed: Dict) -> Dict:
+        """The 8-bit states of what ``state_dict`` has packed as float32 moments."""
         # the packed entries are the live ones of ``self.state``: the float32 moments go into copies, and so does the step
         # count, lest a later step made one of the two older than the other
         params = [p for group in self.param_groups for p in group["params"]]

@@ -457,3 +457,41 @@ def test_differing_counts_leave_the_state_alone(clock):
         with pytest.raises(RuntimeError, match="counts differ"):
             opt.step()
         assert list(opt.state) == [ps[0]] and not Table.made
+
+
+# ---------------------------------------------------------------- state dicts and copies
+
+def _convert_on_the_host(held, entries, to_codes):
+    """Stands for the conversion kernels: what it writes is recognised by the tests."""
+    for st, entry in zip(held, entries):
+        for name in ("exp_avg", "exp_avg_sq"):
+            if to_codes:
+                st[name + "_scale"].fill_(2.0)
+            else:
+                entry[name].fill_(0.25 if name == "exp_avg" else 0.5)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("prepend", [False, True])
+def test_state_dict_hooks_see_float32_moments(bits, prepend, monkeypatch):
+    monkeypatch.setattr(FusedAdam, "_convert_moments", staticmethod(_convert_on_the_host))
+    ps = parameters()
+    opt = FusedAdam(ps, state_bits=bits)
+    give(ps)
+    opt.step()
+    seen = []
+
+    def replace(optimizer, sd):
+        assert optimizer is opt
+        seen.append({i: sorted(st) for i, st in sd["state"].items()})
+        assert all(st[k].dtype == torch.float32 for st in sd["state"].values() for k in ("exp_avg", "exp_avg_sq"))
+        sd["state"][1] = dict(sd["state"][1], exp_avg=torch.full((6,), 7.0))
+
+    handle = opt.register_state_dict_post_hook(replace, prepend=prepend)
+    sd = opt.state_dict()
+    assert seen == [{i: ["exp_avg", "exp_avg_sq", "step"] for i in range(3)}]
+    assert sd["state"][1]["exp_avg"].tolist() == [7.0] * 6 and sorted(sd["state"][0]) == ["exp_avg", "exp_avg_sq", "step"]
+    if bits == 8:
+        assert sd["state"][0]["exp_avg"].tolist() == [0.25] * 4 and opt.state[ps[0]]["exp_avg"].dtype == torch.float8_e4m3fn
+    handle.remove()
+    assert opt.state_dict()["state"][1]["exp_avg"].tolist() == [0.25 if bits == 8 else 0.0] * 6
