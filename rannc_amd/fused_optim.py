@@ -110,8 +110,23 @@ class _Steady:
 
 
 class _FusedBase(torch.optim.Optimizer):
+    #: what a copy (``copy.deepcopy``, pickle) takes along beside torch's own; gate, gradient sources and model copies are
+    #: addresses of the original's surroundings and stay behind
+    _copied: Tuple[str, ...] = ()
+
     def __init__(self, params, defaults):
         super().__init__(params, defaults)
+        self._begin()
+
+    def __getstate__(self) -> Dict:
+        return {**super().__getstate__(), **{name: self.__dict__[name] for name in self._copied}}
+
+    def __setstate__(self, state) -> None:
+        super().__setstate__(state)
+        if "_steady" not in self.__dict__:      # a copy (``load_state_dict`` comes here too)
+            self._begin()
+
+    def _begin(self) -> None:
         self._steady: Dict[int, _Steady] = {}
         self._tables: Dict[Tuple, Tuple[_lib.OptimTable, Tuple, List]] = {}
         self._model_copies: Dict[int, torch.Tensor] = {}
@@ -370,6 +385,7 @@ class FusedAdam(_FusedBase):
     """``torch.optim.Adam`` (amsgrad off) as one launch per parameter group."""
 
     _decoupled = False
+    _copied = ("capturable", "state_bits", "_buffers8")
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, maximize=False,
                  capturable=False, state_bits=32):
@@ -399,13 +415,16 @@ class FusedAdam(_FusedBase):
             raise ValueError("invalid Adam hyper-parameters")
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32, got {state_bits!r}")
-        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, maximize=maximize))
         self.capturable = bool(capturable)
         self.state_bits = int(state_bits)
+        self._buffers8: Dict[int, List[Dict[str, torch.Tensor]]] = {}      # group index -> the buffers its 8-bit states lie in
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, maximize=maximize))
+
+    def _begin(self) -> None:
+        super()._begin()
         if self.state_bits == 8:
             self._conversion_hook = super().register_state_dict_post_hook(FusedAdam._give_moments)
         self._clocks: Dict[int, torch.Tensor] = {}       # group index -> its rg_adam_clock (8 float32 words on the device)
-        self._buffers8: Dict[int, List[Dict[str, torch.Tensor]]] = {}      # group index -> the buffers its 8-bit states lie in
 
     def _make_moments(self, gi: int, params: List[torch.Tensor], loaded: Optional[List[Dict]] = None) -> None:
         """Moments for ``params`` of one group: zeros (with a count of zero where there is none), or in 8 bits what ``loaded``

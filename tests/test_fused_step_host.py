@@ -1,5 +1,8 @@
 """The host side of the fused optimizers' steps without a GPU: which parameters, gradients and counts reach a table, with the
 tables replaced by a record of what they are told.  Each test runs with the compiled module and without it."""
+import copy
+import io
+
 import pytest
 import torch
 
@@ -495,3 +498,44 @@ def test_state_dict_hooks_see_float32_moments(bits, prepend, monkeypatch):
         assert sd["state"][0]["exp_avg"].tolist() == [0.25] * 4 and opt.state[ps[0]]["exp_avg"].dtype == torch.float8_e4m3fn
     handle.remove()
     assert opt.state_dict()["state"][1]["exp_avg"].tolist() == [0.25 if bits == 8 else 0.0] * 6
+
+
+@pytest.mark.parametrize("make", [lambda ps: FusedAdam(ps, lr=0.5), lambda ps: FusedAdamW(ps, state_bits=8), lambda ps: FusedAdam(ps, capturable=True),
+                                  lambda ps: FusedSGD(ps, momentum=0.9)], ids=["adam", "adamw8", "capturable", "sgd"])
+@pytest.mark.parametrize("pickled", [False, True])
+def test_copies_are_optimizers_of_their_own(make, pickled, clock, monkeypatch):
+    monkeypatch.setattr(FusedAdam, "_convert_moments", staticmethod(_convert_on_the_host))
+    ps = parameters()
+    opt = make(ps)
+    for _ in range(2):
+        give(ps)
+        opt.step()
+    if pickled:
+        file = io.BytesIO()
+        torch.save(opt, file)
+        file.seek(0)
+        other = torch.load(file, weights_only=False)       # written here
+    else:
+        other = copy.deepcopy(opt)
+    qs = other.param_groups[0]["params"]
+    assert type(other) is type(opt) and all(q is not p for p, q in zip(ps, qs))
+    a, b = opt.state_dict(), other.state_dict()
+    assert a["param_groups"] == b["param_groups"] and a["state"].keys() == b["state"].keys()
+    for i, st in a["state"].items():
+        assert st.keys() == b["state"][i].keys() and all(torch.equal(v, b["state"][i][k]) for k, v in st.items())
+    if getattr(opt, "state_bits", 32) == 8:
+        assert other.state_bits == 8 and other.state_buffers()["exp_avg"].data_ptr() == other.state[qs[0]]["exp_avg"].data_ptr()
+        assert len(other._optimizer_state_dict_post_hooks) == 1
+    launches = sum(len(t.steps) for t in Table.made)
+    qs = [Param(q.detach()) for q in qs] if pickled else qs       # (a saved parameter is a plain one, which is on the CPU)
+    if pickled:
+        for old, q in zip(other.param_groups[0]["params"], qs):
+            other.state[q] = other.state.pop(old)
+        other.param_groups[0]["params"] = qs
+    give(qs)
+    other.step()
+    assert sum(len(t.steps) for t in Table.made) == launches + 1
+    assert Table.made[-1].params == [q.data_ptr() for q in qs]
+    if isinstance(opt, FusedAdam) and not opt.capturable:
+        assert Table.made[-1].steps[-1][0] == 3 and float(opt.state[ps[0]]["step"]) == 2
+    other.load_state_dict(opt.state_dict())
