@@ -469,6 +469,12 @@ class FusedAdam(_FusedBase):
         if len(held) != 1:
             raise RuntimeError("state_buffers: the group's states are not there yet" if not held else
                                "state_buffers: the group's states came in more than one step and lie in several buffers")
+        ends = {name: (b.data_ptr(), b.data_ptr() + b.numel() * b.element_size()) for name, b in held[0].items()}
+        for p in self.param_groups[group]["params"]:
+            st = self.state.get(p, {})
+            for name, (first, last) in ends.items():
+                if name in st and st[name].numel() and not first <= st[name].data_ptr() < last:
+                    raise RuntimeError(f"state_buffers: a parameter's {name} has been given memory of its own")
         return dict(held[0])
 
     @staticmethod

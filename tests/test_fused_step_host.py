@@ -21,7 +21,7 @@ class Table:
     refuse = None          # an exception that the next launches raise
 
     def __init__(self, device, params, grads, state1, state2, copies, numels, grad_dtypes, copy_dtypes=None, scales1=None, scales2=None):
-        self.params, self.grads, self.state1, self.state2 = list(params), list(grads), state1, state2
+        self.params, self.grads, self.state1, self.state2, self.scales2 = list(params), list(grads), state1, state2, scales2
         self.numels, self.grad_dtypes, self.steps = list(numels), grad_dtypes, []
         self.handle = id(self)
         Table.made.append(self)
@@ -539,3 +539,30 @@ def test_copies_are_optimizers_of_their_own(make, pickled, clock, monkeypatch):
     if isinstance(opt, FusedAdam) and not opt.capturable:
         assert Table.made[-1].steps[-1][0] == 3 and float(opt.state[ps[0]]["step"]) == 2
     other.load_state_dict(opt.state_dict())
+
+
+@pytest.mark.parametrize("name", ["exp_avg", "exp_avg_scale", "exp_avg_sq", "exp_avg_sq_scale"])
+def test_state_buffers_are_where_the_states_lie(name):
+    ps = parameters((4, 0, 300))
+    opt = FusedAdam(ps, state_bits=8)
+    give(ps)
+    opt.step()
+    assert opt.state_buffers()[name].data_ptr() == opt.state[ps[0]][name].data_ptr()
+    opt.state[ps[2]][name] = opt.state[ps[2]][name].clone()
+    with pytest.raises(RuntimeError, match=f"{name} has been given memory"):
+        opt.state_buffers()
+
+
+def test_moved_8_bit_states_get_another_table():
+    """Without ``invalidate_tables``: the states' addresses are compared whenever a step looks at every parameter."""
+    ps = parameters()
+    opt = FusedAdam(ps, state_bits=8)
+    for _ in range(2):
+        give(ps)
+        opt.step()
+    opt.state[ps[1]]["exp_avg_sq_scale"] = opt.state[ps[1]]["exp_avg_sq_scale"].clone()
+    opt._steady.clear()
+    for _ in range(2):
+        opt.step()
+    assert len(Table.made) == 2 and [len(t.steps) for t in Table.made] == [2, 2]
+    assert list(Table.made[1].scales2) == [opt.state[p]["exp_avg_sq_scale"].data_ptr() for p in ps]
