@@ -723,9 +723,10 @@ class FusedSGD(_FusedBase):
                 self._scale_source(table).sgd_step(group["lr"], group["momentum"], group["dampening"], group["weight_decay"],
                                group["nesterov"], group["maximize"], first_step=first, grad_scale=self.grad_scale,
                                gate=self.gate, stream=stream_handle(ps[0].device))
-                if first and made:               # a buffer is the state's once its first step has been launched
-                    for p in ps:
-                        self.state[p]["momentum_buffer"] = made[id(p)]
+                for p in ps:                     # a buffer is the state's once its first step has been launched; without
+                    st = self.state[p]           # momentum a stepped parameter has an empty entry, as in torch.optim
+                    if first:
+                        st["momentum_buffer"] = made[id(p)]
                 if not first and not fresh and len(ps) == len(group["params"]):
                     self._make_steady(gi, group, table, [grad_of[id(p)] for p in ps], None)
         return loss

@@ -566,3 +566,12 @@ def test_moved_8_bit_states_get_another_table():
         opt.step()
     assert len(Table.made) == 2 and [len(t.steps) for t in Table.made] == [2, 2]
     assert list(Table.made[1].scales2) == [opt.state[p]["exp_avg_sq_scale"].data_ptr() for p in ps]
+
+
+@pytest.mark.parametrize("momentum", [0.0, 0.9])
+def test_sgd_state_dict_names_every_stepped_parameter(momentum):
+    ps = parameters()
+    opt = FusedSGD(ps, lr=0.1, momentum=momentum)
+    give(ps[:2])
+    opt.step()
+    assert [sorted(st) for st in opt.state_dict()["state"].values()] == [["momentum_buffer"] if momentum else []] * 2
