@@ -112,9 +112,29 @@ __device__ __forceinline__ float sqrt_normal(float x) {
   return __builtin_fmaf(__builtin_fmaf(-s, s, x), 0.5f * y, s);
 }
 
+__device__ __forceinline__ float minimum3(float a, float b, float c) {       // NaN if any is
+  return __builtin_elementwise_minimum(__builtin_elementwise_minimum(a, b), c);
+}
+
 // Squares are carried times 2^50 and roots times 2^25, so that every square that fp32 holds lies in sqrt_normal's range
-// (a product's factor is moved instead of the product, which costs nothing and changes no rounding).
+// (a product's factor is moved instead of the product, which costs nothing and changes no rounding).  The square of a root
+// that is held in 8 bits (2^-117 at the least) may still lie below it: quick roots under 2^-50 are not used.
 constexpr float kRootShift = 33554432.0f, kSquareShift = 1125899906842624.0f;
+constexpr float kLeastQuickSquare = 7.888609052210118e-31f, kLeastQuickRoot = 8.881784197001252e-16f;    // 2^-100, 2^-50
+
+// The root times 2^25 for any magnitudes: q is the old root times 2^25.  Every product is rounded as if exponents had no end:
+// what leaves fp32's range times 2^50 is worked out times 1 or times 2^200.
+__device__ __forceinline__ float root_of_any(float q, float g, float beta2, float one_minus_beta2) {
+  const float square = beta2 * (q * q) + ((one_minus_beta2 * kSquareShift) * g) * g;
+  if (square < kLeastQuickSquare) {
+    const float old = fminf(q, 67108864.0f) * 137438953472.0f;            // 2^37; the minimum is q, unless beta2 is 0
+    const float grad = g * 1.2676506002282294e30f;                        // 2^100
+    return sqrtf((beta2 * 7.555786372591432e22f) * (old * old) + (one_minus_beta2 * grad) * grad) * 2.6469779601696886e-23f;   // 2^76, 2^-75
+  }
+  if (square < __builtin_inff()) return sqrtf(square);
+  const float old = q * (1.0f / kRootShift);
+  return sqrtf(beta2 * (old * old) + (one_minus_beta2 * g) * g) * kRootShift;
+}
 
 // One block of 256 elements (fewer at a tensor's end) by one wavefront, four per lane:
 //   m = beta1 m + (1 - beta1) g,  v = beta2 r^2 + (1 - beta2) g^2,  r = sqrt(v),  p -= step_size m / (r / bias2_sqrt + eps)
@@ -160,15 +180,13 @@ __device__ __forceinline__ void adam8_block(const Opt8ChunkRec& r, int start, in
     root[j] = sqrt_normal(c.beta2 * (q[j] * q[j]) + (one_minus_beta2 * g[j]) * g[j]);
   }
   float top2 = __builtin_elementwise_maximum(maximum_abs3(root[0], root[1], root[2]), root[3]);
-  const bool plain = __builtin_amdgcn_ballot_w64(top2 != top2) == 0;
-  if (!plain) {      // some second moment is zero, subnormal or not a number: the roots one by one
+  const float low2 = __builtin_elementwise_minimum(minimum3(root[0], root[1], root[2]), root[3]);
+  const bool plain = __builtin_amdgcn_ballot_w64(!(low2 >= kLeastQuickRoot)) == 0;
+  if (!plain) {      // some second moment is zero, very small or not a number: the roots one by one
     top2 = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float square = c.beta2 * (q[j] * q[j]) + (one_minus_beta2 * g[j]) * g[j];
-      const float old = q[j] * (1.0f / kRootShift);      // the shift may have made it infinite
-      root[j] = square < __builtin_inff() ? sqrtf(square)
-                                          : sqrtf(c.beta2 * (old * old) + (c.one_minus_beta2 * g[j]) * g[j]) * kRootShift;
+      root[j] = root_of_any(q[j], g[j], c.beta2, c.one_minus_beta2);
       top2 = __builtin_elementwise_maximum(top2, __builtin_fabsf(root[j]));
     }
   }
