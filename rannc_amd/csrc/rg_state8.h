@@ -56,7 +56,8 @@ __device__ __forceinline__ BlockScale block_scale(uint32_t max_bits, float shift
   const bool number = max_bits < 0x7f800000u, holds = number && s >= __uint_as_float(kState8TinyBits);
   BlockScale out;
   out.s = holds ? s : number ? 0.0f : __uint_as_float(0x7fc00000u);
-  out.inv = holds ? 256.0f * (1.0f / top) : 0.0f;       // 1 / top correctly rounded: top * inv rounds to 256 at most
+  // 256 / top correctly rounded, so that top * inv rounds to 256 at most.  (1 / top, taken first, is subnormal from 2^126 on.)
+  out.inv = holds ? 1.0f / (top * 0.00390625f) : 0.0f;
   return out;
 }
 

@@ -4,9 +4,11 @@ import pytest
 import torch
 
 from oracle import state8 as oracle
+from rannc_amd.multi_tensor import State8Plan, allocate_state8
 from tests.test_gpu_state8 import KW, Step, launch
 
 pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
 
 
 def small_state(rng, exponents, zero_gradients):
@@ -59,3 +61,25 @@ def test_a_small_root_decays_without_vanishing():
         elif want < 2.0 ** -100 * 0.99:
             assert s == 0.0 and not t.dc2[0].any(), step
     t.table.close()
+
+
+@pytest.mark.parametrize("mantissa", [1.5, 1.75, 1.0 + 2.0 ** -23, 1.6180339887, 2.0 - 2.0 ** -23])
+def test_codes_do_not_depend_on_the_power_of_two(mantissa):
+    """The same block times 2^e, from 2^-100 up to fp32's largest numbers, with halfway numbers among its elements: the reciprocal of
+    the scale has to keep its 24 bits everywhere."""
+    grid = oracle.GRID[:oracle.GRID.searchsorted(256.0) + 1]
+    y = np.concatenate([[256.0], (grid[1:] + grid[:-1]) / 2, grid, -grid[100:114]])[:256]
+    mantissa = float(np.float32(mantissa))
+    block = (y / 256 * mantissa).astype(np.float32)            # numbers from 2^-18 to 2: no exponent below makes them subnormal,
+    exponents = [0, 127, 126, 125, 124, 60, -60, -99]          # but the last one's smallest
+    x = np.concatenate([np.ldexp(block, e) for e in exponents])
+    v = torch.from_numpy(x).to(DEV)
+    codes, scales, _, _ = allocate_state8([v])
+    plan = State8Plan([v], codes, scales)
+    plan.quantize()
+    assert scales[0].tolist() == [float(np.ldexp(mantissa, e)) for e in exponents]
+    got = codes[0].view(torch.uint8).cpu().numpy().reshape(len(exponents), 256)
+    assert y.size == 256 and (got == got[0]).all(), np.argwhere(got != got[0])
+    if mantissa == 1.5:             # the reciprocal's rounding moves no halfway number here: ties to even, as the oracle has them
+        assert np.array_equal(got[0], oracle.quantize(block.astype(np.float64), False)[0])
+    plan.close()
