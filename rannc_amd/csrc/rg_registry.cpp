@@ -21,11 +21,9 @@ using namespace rgbind;
 
 namespace {
 
-// Whether a gradient can be a row of an optimizer table as it is, and its address appended if so.  With an owner it has to be
-// of the owner's size and on its device as well.
-bool append_address(const at::Tensor& g, at::ScalarType dtype, std::string& out, const at::Tensor* owner = nullptr) {
+// Whether a gradient can be a row of an optimizer table as it is, and its address appended if so.
+bool append_address(const at::Tensor& g, at::ScalarType dtype, std::string& out) {
   if (!g.defined() || g.layout() != at::kStrided || g.scalar_type() != dtype || !g.is_contiguous()) return false;
-  if (owner != nullptr && (!owner->defined() || g.numel() != owner->numel() || g.device() != owner->device())) return false;
   const uintptr_t address = reinterpret_cast<uintptr_t>(g.numel() ? g.const_data_ptr() : nullptr);
   out.append(reinterpret_cast<const char*>(&address), sizeof(address));
   return true;
@@ -36,6 +34,8 @@ bool append_address(const at::Tensor& g, at::ScalarType dtype, std::string& out,
 class TensorList {
  public:
   explicit TensorList(const py::object& tensors) : t_(tensor_vector(tensors, "TensorList")) {
+    rows_.reserve(t_.size());
+    for (const at::Tensor& t : t_) rows_.push_back(t.defined() ? Row{t.numel(), t.device()} : Row{-1, at::kCPU});
     if (!PyList_Check(tensors.ptr()) && !PyTuple_Check(tensors.ptr())) return;
     objects_.reserve(t_.size());
     for (const py::handle& o : tensors) objects_.push_back(py::reinterpret_borrow<py::object>(o));
@@ -73,13 +73,13 @@ class TensorList {
     if (views.size() != t_.size()) throw std::invalid_argument("set_grads: the lists differ in length");
     for (size_t i = 0; i < t_.size(); ++i) t_[i].mutable_grad() = views.t_[i];
   }
-  // The addresses of all gradients, one machine word each; None unless every tensor has a contiguous one of `dtype`, of its size
-  // and on its device.
+  // The addresses of all gradients, one machine word each; None unless every tensor has a contiguous one of `dtype`, of the size
+  // and on the device that the tensor had when the list was made of it (what a table made at that time knows).
   py::object grad_addresses(at::ScalarType dtype) const {
     std::string out;
     out.reserve(t_.size() * sizeof(uintptr_t));
-    for (const at::Tensor& t : t_)
-      if (!t.defined() || !append_address(t.grad(), dtype, out, &t)) return py::none();
+    for (size_t i = 0; i < t_.size(); ++i)
+      if (!t_[i].defined() || !append_row(i, t_[i].grad(), dtype, out)) return py::none();
     return py::bytes(out);
   }
   // The same for gradients that are given, one for each tensor.
@@ -88,7 +88,7 @@ class TensorList {
     std::string out;
     out.reserve(t_.size() * sizeof(uintptr_t));
     for (size_t i = 0; i < t_.size(); ++i)
-      if (!append_address(tensor_or_undefined(grads[i], "addresses_of"), dtype, out, &t_[i])) return py::none();
+      if (!append_row(i, tensor_or_undefined(grads[i], "addresses_of"), dtype, out)) return py::none();
     return py::bytes(out);
   }
   void clear_grads() {
@@ -112,8 +112,17 @@ class TensorList {
   }
 
  private:
+  struct Row {
+    int64_t numel;
+    at::Device device;
+  };
+  bool append_row(size_t i, const at::Tensor& g, at::ScalarType dtype, std::string& out) const {
+    return i < rows_.size() && g.defined() && g.numel() == rows_[i].numel && g.device() == rows_[i].device && append_address(g, dtype, out);
+  }
+
   std::vector<at::Tensor> t_;
   std::vector<py::object> objects_;
+  std::vector<Row> rows_;
 };
 
 // ------------------------------------------------------------------------------------------------ GradPlan
@@ -794,7 +803,7 @@ void bind_registry(py::module_& m) {
       .def("grads", &TensorList::grads)
       .def("grad_addresses", [](const TensorList& l, const py::object& dtype) {
              return l.grad_addresses(torch::python::detail::py_object_to_dtype(dtype));
-           }, "the gradients' addresses as packed machine words; None unless every tensor has a contiguous gradient of `dtype`, of its size and on its device")
+           }, "the gradients' addresses as packed machine words; None unless every tensor has a contiguous gradient of `dtype`, of the size and on the device that it had when the list was made")
       .def("addresses_of", [](const TensorList& l, const py::list& grads, const py::object& dtype) {
              return l.addresses_of(grads, torch::python::detail::py_object_to_dtype(dtype));
            }, "grad_addresses for gradients that are given, one for each tensor (None: it has none)")

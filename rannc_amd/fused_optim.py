@@ -90,7 +90,7 @@ class _Steady:
     """What a group's last full step established, for the steps after it: as long as the same parameters all
     have contiguous gradients of the same dtype, a step is one pointer comparison per gradient and one launch."""
     __slots__ = ("params", "n", "param_ids", "table", "key", "grad_ptrs", "grad_dtype", "steps_buf", "steps_np", "count", "device",
-                 "param_ptr_ends", "fed_by")
+                 "param_ptr_ends", "fed_by", "numels")
 
     def same(self, params: List[torch.Tensor], first: int = 0) -> bool:
         """Whether ``params`` holds the record's very parameters from ``first`` on."""
@@ -100,11 +100,11 @@ class _Steady:
 
     def addresses(self, grads: Optional[List[Optional[torch.Tensor]]] = None) -> Optional[bytes]:
         """Where the gradients lie (those given, or the parameters' own); None unless each parameter has one that the table
-        can read."""
+        can read, that is also of the size the table was made for."""
         if type(self.params) is not tuple:
             return self.params.grad_addresses(self.grad_dtype) if grads is None else self.params.addresses_of(grads, self.grad_dtype)
         grads = [p.grad for p in self.params] if grads is None else grads
-        if any(g is not None and (g.numel() != p.numel() or g.device != p.device) for g, p in zip(grads, self.params)):
+        if any(g is not None and (g.numel() != n or g.device != self.device) for g, n in zip(grads, self.numels)):
             return None
         return _addresses(grads, self.grad_dtype)
 
@@ -259,7 +259,8 @@ class _FusedBase(torch.optim.Optimizer):
     def _make_steady(self, gi: int, group, table, grads: List[torch.Tensor], count: Optional[int]) -> None:
         params = group["params"]
         st = _Steady()
-        st.params, st.n = self._native_list(gi, params) if _native is not None else tuple(params), len(params)
+        st.params, st.n = _native.TensorList(params) if _native is not None else tuple(params), len(params)
+        st.numels = table.cache_key[-1]
         st.param_ids = [id(p) for p in params]
         st.table = table
         st.key = table.cache_key
@@ -634,14 +635,20 @@ class FusedAdam(_FusedBase):
                 self._check_param(p, g)
                 found.append(p)
                 grad_of[id(p)] = g
-            self._make_moments(gi, [p for p in found if "exp_avg" not in self.state.get(p, {})])
+            held = [self.state.get(p) for p in found]         # (a tensor's hash is a call into Python: looked up once)
+            fresh = [p for p, st in zip(found, held) if st is None or "exp_avg" not in st]
+            self._make_moments(gi, fresh)
             self._settle_moments(gi, group["params"])
-            for p in found:
+            if fresh:
+                held = [self.state[p] for p in found]
+            count_of: Dict[int, torch.Tensor] = {}
+            for p, st in zip(found, held):
                 # ``step`` stays a tensor (torch.optim's state layout); its integer value is mirrored
                 # here so that a step costs one batched increment instead of one tensor op per parameter
-                t = self.state[p]["step"]
+                t = st["step"]
                 if not torch.is_tensor(t):
-                    t = self.state[p]["step"] = torch.tensor(float(t), dtype=torch.float32)
+                    t = st["step"] = torch.tensor(float(t), dtype=torch.float32)
+                count_of[id(p)] = t
                 seen = self._steps.get(id(p))
                 by_step.setdefault((seen[1] if seen is not None and seen[0] is t else int(t)) + 1, []).append(p)
             tables = [self._table((gi, tuple(id(p) for p in ps)), ps, [grad_of[id(p)] for p in ps], *self._moments(ps))
@@ -651,7 +658,7 @@ class FusedAdam(_FusedBase):
                 self._scale_source(table).adam_step(group["lr"], b1, b2, group["eps"], group["weight_decay"], step,
                                 decoupled=self._decoupled, maximize=group["maximize"], grad_scale=self.grad_scale,
                                 gate=self.gate, stream=stream_handle(ps[0].device))
-                counts = [self.state[p]["step"] for p in ps]          # ... and the counts move behind it
+                counts = [count_of[id(p)] for p in ps]                # ... and the counts move behind it
                 torch._foreach_add_(counts, 1)
                 self._steps.update((id(p), (t, step)) for p, t in zip(ps, counts))
                 if len(by_step) == 1 and len(ps) == len(group["params"]):

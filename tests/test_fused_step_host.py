@@ -575,3 +575,19 @@ def test_sgd_state_dict_names_every_stepped_parameter(momentum):
     give(ps[:2])
     opt.step()
     assert [sorted(st) for st in opt.state_dict()["state"].values()] == [["momentum_buffer"] if momentum else []] * 2
+
+
+def test_a_parameter_resized_between_the_ends_leaves_the_short_path():
+    """Its gradient is then of another size than the table's row, whatever the parameter's size is by now."""
+    ps = parameters()
+    opt = FusedSGD(ps, lr=0.1)
+    for _ in range(3):
+        give(ps)
+        opt.step()
+    ps[1].grad = None
+    ps[1].data = torch.zeros(9)
+    for _ in range(3):
+        give(ps)
+        opt.step()
+        assert Table.made[-1].numels == [4, 9, 5] and Table.made[-1].steps[-1][1:] == ([p.data_ptr() for p in ps], [p.grad.data_ptr() for p in ps])
+    assert len(Table.made) == 2 and [len(t.steps) for t in Table.made] == [3, 3]
