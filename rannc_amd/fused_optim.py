@@ -393,7 +393,9 @@ class FusedAdam(_FusedBase):
         """``state_bits=8``: both moments are held in 8 bits (``ranncgrad.h``, "optimizer states in 8 bits"): a byte an
         element and a float32 scale for every 256 of them, a quarter of the moments' memory and traffic.  exp_avg_sq is
         held as its root, and a step rounds with a dither that depends on the step count and the element's place alone,
-        so that a run can be repeated bit for bit.  ``state[p]`` then has the codes under ``exp_avg`` / ``exp_avg_sq``
+        so that a run can be repeated bit for bit.  Over a run exp_avg_sq comes out 4-8 % too large and single roots 15-20 % (rms)
+        off the float32 ones; the same gradients move parameters as with 32 bits but for about 1 % in length and an angle of 4
+        degrees (2,000 steps).  ``state[p]`` then has the codes under ``exp_avg`` / ``exp_avg_sq``
         and the scales under ``exp_avg_scale`` / ``exp_avg_sq_scale``; ``state_dict()`` gives, and ``load_state_dict()``
         takes, the float32 moments of ``torch.optim.Adam`` - converted on the GPU, which holds both forms meanwhile.  What
         ``state_dict()`` gave loads back as the same codes and scales (but for about one block in two million, see

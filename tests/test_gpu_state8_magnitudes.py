@@ -83,3 +83,28 @@ def test_codes_do_not_depend_on_the_power_of_two(mantissa):
     if mantissa == 1.5:             # the reciprocal's rounding moves no halfway number here: ties to even, as the oracle has them
         assert np.array_equal(got[0], oracle.quantize(block.astype(np.float64), False)[0])
     plan.close()
+
+
+def test_square_root_of_every_number():
+    """All fp32 numbers from the smallest up to 2^78, one to a block of equal ones (the scale is then the root, and no zero sends the
+    block another way): the quick square root is correctly rounded over its whole range, 2^-100 to infinity after the factor of
+    2^50.  The root in float64 rounds to fp32 as the exact one does (53 >= 2 * 24 + 2)."""
+    count = 1 << 20
+    values = torch.empty(count * 256, device=DEV)
+    codes, scales, _, _ = allocate_state8([values])
+    plan = State8Plan([values], codes, scales, root=True)
+    end = (127 + 78) << 23
+    offsets = torch.arange(count, dtype=torch.int32, device=DEV)
+    wrong = torch.zeros((), dtype=torch.int64, device=DEV)
+    for first in range(1, end, count):
+        bits = torch.clamp(offsets + first, max=end - 1)
+        x = bits.view(torch.float32)
+        values.view(count, 256).copy_(x.unsqueeze(1).expand(count, 256))
+        plan.quantize()
+        # subnormal numbers by their bits: no conversion flushes them
+        exact = torch.where(bits < 1 << 23, bits.double() * 2.0 ** -149, x.double())
+        want = exact.sqrt().float()
+        wrong += (scales[0].view(torch.int32) != want.view(torch.int32)).sum()
+    assert int(wrong) == 0
+    assert bool((codes[0].view(torch.uint8) == 0x78).all())          # 256: the largest of its block
+    plan.close()
