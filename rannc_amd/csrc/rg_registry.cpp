@@ -82,6 +82,11 @@ class TensorList {
       if (!t_[i].defined() || !append_row(i, t_[i].grad(), dtype, out)) return py::none();
     return py::bytes(out);
   }
+  // grad_addresses() if `tensors` holds this list's very objects and no others.
+  py::object grad_addresses_in(const py::sequence& tensors, at::ScalarType dtype) const {
+    if ((size_t)PySequence_Size(tensors.ptr()) != t_.size() || !holds(tensors, 0)) return py::none();
+    return grad_addresses(dtype);
+  }
   // The same for gradients that are given, one for each tensor.
   py::object addresses_of(const py::list& grads, at::ScalarType dtype) const {
     if (grads.size() != t_.size()) return py::none();
@@ -804,6 +809,9 @@ void bind_registry(py::module_& m) {
       .def("grad_addresses", [](const TensorList& l, const py::object& dtype) {
              return l.grad_addresses(torch::python::detail::py_object_to_dtype(dtype));
            }, "the gradients' addresses as packed machine words; None unless every tensor has a contiguous gradient of `dtype`, of the size and on the device that it had when the list was made")
+      .def("grad_addresses_in", [](const TensorList& l, const py::sequence& tensors, const py::object& dtype) {
+             return l.grad_addresses_in(tensors, torch::python::detail::py_object_to_dtype(dtype));
+           }, "grad_addresses if `tensors` is a list or tuple of the very objects this list was made of")
       .def("addresses_of", [](const TensorList& l, const py::list& grads, const py::object& dtype) {
              return l.addresses_of(grads, torch::python::detail::py_object_to_dtype(dtype));
            }, "grad_addresses for gradients that are given, one for each tensor (None: it has none)")

@@ -98,12 +98,11 @@ class _Steady:
             return self.params.holds(params, first)
         return first + self.n <= len(params) and all(map(is_, self.params, params[first:]))
 
-    def addresses(self, grads: Optional[List[Optional[torch.Tensor]]] = None) -> Optional[bytes]:
-        """Where the gradients lie (those given, or the parameters' own); None unless each parameter has one that the table
-        can read, that is also of the size the table was made for."""
+    def addresses(self, grads: List[Optional[torch.Tensor]]) -> Optional[bytes]:
+        """Where the parameters' gradients lie; None unless each parameter has one that the table can read, that is also of
+        the size the table was made for."""
         if type(self.params) is not tuple:
-            return self.params.grad_addresses(self.grad_dtype) if grads is None else self.params.addresses_of(grads, self.grad_dtype)
-        grads = [p.grad for p in self.params] if grads is None else grads
+            return self.params.addresses_of(grads, self.grad_dtype)
         if any(g is not None and (g.numel() != n or g.device != self.device) for g, n in zip(grads, self.numels)):
             return None
         return _addresses(grads, self.grad_dtype)
@@ -216,9 +215,11 @@ class _FusedBase(torch.optim.Optimizer):
         the group differs from the step that made the record (then the full path runs and makes a new one)."""
         st = self._steady.get(gi)
         params = group["params"]
-        if st is None or len(params) != st.n or not st.same(params):
+        if st is None or len(params) != st.n:
             return None
         if self._feed is not None and not self._grad_sources:
+            if not st.same(params):
+                return None
             off = self._feed_offsets.get(gi) if self._feed_offsets is not None else None
             if (off is not None and st.same(self._feed_params, off) and self._feed.held() >= off + st.n and dtype_code(st.grad_dtype) == self._feed.source_dtype()
                     and (params[0].data_ptr(), params[-1].data_ptr()) == st.param_ptr_ends):
@@ -238,10 +239,14 @@ class _FusedBase(torch.optim.Optimizer):
         # looked at here, code that re-homes others calls ``invalidate_tables``
         if (params[0].data_ptr(), params[-1].data_ptr()) != st.param_ptr_ends:
             return None
-        if self._grad_sources:
+        if not self._grad_sources and type(st.params) is not tuple:
+            found = st.params.grad_addresses_in(params, st.grad_dtype)
+        elif not st.same(params):
+            return None
+        elif self._grad_sources:
             found = st.addresses(list(map(self._grad_sources.get, st.param_ids)))
         else:
-            found = st.addresses()
+            found = st.addresses([p.grad for p in params])
         if found is None:
             return None
         if found != st.grad_ptrs:

@@ -591,3 +591,17 @@ def test_a_parameter_resized_between_the_ends_leaves_the_short_path():
         opt.step()
         assert Table.made[-1].numels == [4, 9, 5] and Table.made[-1].steps[-1][1:] == ([p.data_ptr() for p in ps], [p.grad.data_ptr() for p in ps])
     assert len(Table.made) == 2 and [len(t.steps) for t in Table.made] == [3, 3]
+
+
+def test_addresses_of_the_very_list():
+    native = fused_optim._native
+    if native is None:
+        pytest.skip("the compiled module is switched off")
+    ps = parameters()
+    held = native.TensorList(ps)
+    give(ps)
+    want = held.grad_addresses(torch.float32)
+    assert want is not None and held.grad_addresses_in(ps, torch.float32) == want == held.grad_addresses_in(tuple(ps), torch.float32)
+    for other in (ps + ps[:1], ps[:2], ps[::-1], [ps[0], ps[1].detach(), ps[2]], []):
+        assert held.grad_addresses_in(other, torch.float32) is None
+    assert held.grad_addresses_in(ps, torch.float16) is None
