@@ -18,7 +18,7 @@ from typing import Dict, List, Optional, Tuple
 import torch
 
 from . import _lib
-from .multi_tensor import State8Plan, allocate_state8, dtype_code, stream_handle
+from .multi_tensor import _CODES, State8Plan, allocate_state8, dtype_code, stream_handle
 
 try:        # the compiled module: lists of parameters walked in C++
     from . import _ranncgrad as _native
@@ -27,6 +27,7 @@ except ImportError:
 
 
 _data_ptr = torch.Tensor.data_ptr
+_numel = torch.Tensor.numel
 
 
 def _packed(tensors) -> bytes:
@@ -330,7 +331,8 @@ class _FusedBase(torch.optim.Optimizer):
             raise ValueError("sparse gradients are not supported")
         if not g.is_contiguous() or g.device != p.device or g.numel() != p.numel():
             raise ValueError("gradient must be contiguous, on the parameter's device and of its size")
-        dtype_code(g.dtype)
+        if g.dtype not in _CODES:
+            dtype_code(g.dtype)
 
     @staticmethod
     def _check_rows(params, copies, state1, state2, scales) -> None:
@@ -356,12 +358,12 @@ class _FusedBase(torch.optim.Optimizer):
         """Table for this exact list of parameters and gradient dtypes, re-pointed when any address moved.  ``scales``:
         the states are in 8 bits, and these are their blocks' scales."""
         copies = [self._model_copies.get(id(p)) for p in params]
-        key = key + (tuple(g.dtype for g in grads), tuple(p.numel() for p in params))      # what a table cannot change
-        ptrs = (tuple(p.data_ptr() for p in params), tuple(g.data_ptr() for g in grads),
-                tuple(s.data_ptr() for s in state1) if state1 is not None else None,
-                tuple(s.data_ptr() for s in state2) if state2 is not None else None,
-                tuple(c.data_ptr() if c is not None else 0 for c in copies))
-        scale_ptrs = tuple(tuple(s.data_ptr() for s in part) for part in scales) if scales is not None else (None, None)
+        key = key + (tuple([g.dtype for g in grads]), tuple(map(_numel, params)))      # what a table cannot change
+        def addresses(tensors):
+            return tuple(map(_data_ptr, tensors)) if tensors is not None else None
+        ptrs = (addresses(params), addresses(grads), addresses(state1), addresses(state2),
+                tuple([c.data_ptr() if c is not None else 0 for c in copies]))
+        scale_ptrs = tuple(map(addresses, scales)) if scales is not None else (None, None)
         ptrs += scale_ptrs
         hit = self._tables.get(key)
         dev = params[0].device
@@ -632,7 +634,7 @@ class FusedAdam(_FusedBase):
                 st.steps_np += 1.0
                 continue
             self._steady.pop(gi, None)
-            by_step: Dict[int, List[torch.Tensor]] = {}
+            by_step: Dict[int, Tuple[List[torch.Tensor], List[torch.Tensor]]] = {}       # count -> parameters, their counts
             grad_of: Dict[int, torch.Tensor] = {}
             found = []
             for p in group["params"]:            # everything that can be refused or fail comes before the first launch,
@@ -648,26 +650,26 @@ class FusedAdam(_FusedBase):
             self._settle_moments(gi, group["params"])
             if fresh:
                 held = [self.state[p] for p in found]
-            count_of: Dict[int, torch.Tensor] = {}
             for p, st in zip(found, held):
                 # ``step`` stays a tensor (torch.optim's state layout); its integer value is mirrored
                 # here so that a step costs one batched increment instead of one tensor op per parameter
                 t = st["step"]
-                if not torch.is_tensor(t):
+                if not isinstance(t, torch.Tensor):
                     t = st["step"] = torch.tensor(float(t), dtype=torch.float32)
-                count_of[id(p)] = t
                 seen = self._steps.get(id(p))
-                by_step.setdefault((seen[1] if seen is not None and seen[0] is t else int(t)) + 1, []).append(p)
-            tables = [self._table((gi, tuple(id(p) for p in ps)), ps, [grad_of[id(p)] for p in ps], *self._moments(ps))
-                      for ps in by_step.values()]
-            for table, (step, ps) in zip(tables, by_step.items()):
+                ps, counts = by_step.setdefault((seen[1] if seen is not None and seen[0] is t else int(t)) + 1, ([], []))
+                ps.append(p)
+                counts.append(t)
+            tables = [self._table((gi, tuple(map(id, ps))), ps, [grad_of[id(p)] for p in ps], *self._moments(ps))
+                      for ps, _ in by_step.values()]
+            for table, (step, (ps, counts)) in zip(tables, by_step.items()):
                 b1, b2 = group["betas"]
                 self._scale_source(table).adam_step(group["lr"], b1, b2, group["eps"], group["weight_decay"], step,
                                 decoupled=self._decoupled, maximize=group["maximize"], grad_scale=self.grad_scale,
                                 gate=self.gate, stream=stream_handle(ps[0].device))
-                counts = [count_of[id(p)] for p in ps]                # ... and the counts move behind it
-                torch._foreach_add_(counts, 1)
-                self._steps.update((id(p), (t, step)) for p, t in zip(ps, counts))
+                torch._foreach_add_(counts, 1)                        # ... and the counts move behind it
+                for p, t in zip(ps, counts):
+                    self._steps[id(p)] = (t, step)
                 if len(by_step) == 1 and len(ps) == len(group["params"]):
                     self._make_steady(gi, group, table, [grad_of[id(p)] for p in ps], step)
         return loss
@@ -709,8 +711,8 @@ class FusedSGD(_FusedBase):
                                   gate=self.gate, stream=stream_handle(st.device))
                 continue
             self._steady.pop(gi, None)
-            fresh, seasoned = [], []
-            made: Dict[int, torch.Tensor] = {}
+            fresh, seasoned, unnamed = [], [], []
+            buffer_of: Dict[int, torch.Tensor] = {}
             grad_of: Dict[int, torch.Tensor] = {}
             for p in group["params"]:
                 g = self._grad_of(p)
@@ -718,29 +720,34 @@ class FusedSGD(_FusedBase):
                     continue
                 self._check_param(p, g)
                 grad_of[id(p)] = g
-                if group["momentum"] != 0 and self.state.get(p, {}).get("momentum_buffer") is None:
+                st = self.state.get(p)
+                buffer = st.get("momentum_buffer") if st is not None else None
+                if group["momentum"] != 0 and buffer is None:
                     # zeros, not empty: if the first launch is gated off on the device the buffer must
                     # not reach the next step with whatever the memory held
-                    made[id(p)] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                    buffer = torch.zeros_like(p, memory_format=torch.preserve_format)
                     fresh.append(p)
                 else:
                     seasoned.append(p)
+                    if st is None:
+                        unnamed.append(p)
+                buffer_of[id(p)] = buffer
             tables = []                          # all of them before the first launch: what fails leaves the state as it was
             for first, ps in ((True, fresh), (False, seasoned)):
                 if not ps:
                     continue
-                bufs = None
-                if group["momentum"] != 0:
-                    bufs = [made[id(p)] if first else self.state[p]["momentum_buffer"] for p in ps]
-                tables.append((first, ps, self._table((gi, first, tuple(id(p) for p in ps)), ps, [grad_of[id(p)] for p in ps], bufs, None)))
+                bufs = [buffer_of[id(p)] for p in ps] if group["momentum"] != 0 else None
+                tables.append((first, ps, self._table((gi, first, tuple(map(id, ps))), ps, [grad_of[id(p)] for p in ps], bufs, None)))
             for first, ps, table in tables:
                 self._scale_source(table).sgd_step(group["lr"], group["momentum"], group["dampening"], group["weight_decay"],
                                group["nesterov"], group["maximize"], first_step=first, grad_scale=self.grad_scale,
                                gate=self.gate, stream=stream_handle(ps[0].device))
-                for p in ps:                     # a buffer is the state's once its first step has been launched; without
-                    st = self.state[p]           # momentum a stepped parameter has an empty entry, as in torch.optim
-                    if first:
-                        st["momentum_buffer"] = made[id(p)]
+                if first:                        # a buffer is the state's once its first step has been launched
+                    for p in ps:
+                        self.state[p]["momentum_buffer"] = buffer_of[id(p)]
+                else:
+                    for p in unnamed:            # without momentum a stepped parameter has an empty entry, as in torch.optim
+                        self.state[p]
                 if not first and not fresh and len(ps) == len(group["params"]):
                     self._make_steady(gi, group, table, [grad_of[id(p)] for p in ps], None)
         return loss
