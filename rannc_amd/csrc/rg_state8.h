@@ -98,8 +98,9 @@ template <bool NT> __device__ __forceinline__ void st_codes(char* p, uint32_t w)
   if (NT) __builtin_nontemporal_store(w, g);
   else *g = w;
 }
-// A block's scale, the same address for all lanes: through a pointer of the global address space, so that it becomes a
-// scalar load (a generic pointer compiles to a FLAT load, whose wait drains every load in flight).
+// A block's scale, the same address for all lanes: through a pointer of the global address space it becomes a scalar load, through
+// a generic one a FLAT load, whose wait drains every load in flight.  The step takes the same time either way.  (A scale is read
+// before its block's wavefront, and no other, writes it; the scalar cache starts empty in every launch.)
 __device__ __forceinline__ float load_scale(const float* p) { return *(const RG_GLOBAL float*)p; }
 __device__ __forceinline__ uint32_t load_u8(const char* p) { return (uint32_t)*(const RG_GLOBAL unsigned char*)p; }
 

@@ -69,7 +69,9 @@ template <bool NT> __device__ __forceinline__ void store_codes4(char* p, int n, 
 // Hand-out order of a launch's tiles: workgroups are dealt to the eight XCDs in turn, and runs of consecutive tiles go to
 // one of them (an incomplete last round keeps its order).  The step, BERT-large in bf16 / 621 M elements in fp16 / 934 ResNet tensors in
 // fp32, by run: 16: 909 / 1,716 / 604 us, 64: 884 / 1,666 / 581, 128: 864 / 1,655 / 585, 224: 860 / 1,630 / 590,
-// 448: 867 / 1,621 / 592.  The conversions over bare arrays: reading back 259 us in turn and 247 in runs of 64, quantizing 263 and 262.
+// 448: 867 / 1,621 / 592.  From 128 to 448 each stays within 2 % of its best; 224 and 448 have the least sum, and 224 keeps the order
+// of shorter tables.  The conversions over bare arrays: reading back 259 us in turn and 247 in runs of 64; quantizing does not care (263
+// and 262) and takes the same run.
 constexpr unsigned kXcdRun = 224;
 constexpr unsigned kConvXcdRun = 64;
 template <unsigned RUN> __device__ __forceinline__ unsigned tile_of_block() {
@@ -105,7 +107,8 @@ __device__ __forceinline__ float maximum_abs3(float a, float b, float c) {   // 
 
 // Square root in five instructions (the compiler's own takes 15), correctly rounded, for 2^-100 <= x < infinity; NaN for anything smaller than 2^-126 (zero too) and for
 // infinity.  The estimate x * rsq(x) is off by at most a few units; its residual x - s^2 is exact in one fma, and s +
-// residual / (2 s) then rounds as the root itself does: checked for every fp32 number of the range.
+// residual / (2 s) then rounds as the root itself does: tests/test_gpu_state8_magnitudes.py compares every number of the
+// range with the root in float64.
 __device__ __forceinline__ float sqrt_normal(float x) {
   const float y = __builtin_amdgcn_rsqf(x);
   const float s = x * y;
@@ -140,9 +143,11 @@ __device__ __forceinline__ float root_of_any(float q, float g, float beta2, floa
 //   m = beta1 m + (1 - beta1) g,  v = beta2 r^2 + (1 - beta2) g^2,  r = sqrt(v),  p -= step_size m / (r / bias2_sqrt + eps)
 // and m and r back to codes by their new largest magnitudes.  Every operation that a code depends on is rounded by itself,
 // so the codes are those of the same formulas written in elementary fp32 operations; the parameter's quotient is not
-// (a reciprocal of 1 unit).  About 45 vector instructions an element: 858 us for 5.38 GB (6.3 TB/s), and 863 us, that is the same,
-// in builds without the square root, the encoding or the reduction: HBM with six streams read and written bounds it
-// (838-852 us for those streams over bare arrays without a table).
+// (a reciprocal of 1 unit).  About 52 vector instructions an element: 858-870 us for 5.38 GB (6.2-6.3 TB/s), and the same in builds
+// without the square root, the encoding or the reduction: HBM with six streams read and written bounds it (838-852 us for those
+// streams over bare arrays without a table).  Those figures are for tensors that begin at multiples of 256 elements.  A block lies
+// where its tensor puts it, so on others the parameter's and copy's accesses straddle lines: 1,097 us with tensors 16 elements further on,
+// 1,200 us with tensors 1 or 3 elements further on.
 template <int G, int C, bool NT, bool FULL>
 __device__ __forceinline__ void adam8_block(const Opt8ChunkRec& r, int start, int lane, const Adam8Const& c, float coef,
                                             uint32_t step) {
@@ -356,7 +361,8 @@ __device__ __forceinline__ void quantize_pair(const State8Rec& r, int start, int
 }
 
 // Back to fp32, two blocks a wavefront with both loads first: 253 us for 1.68 GB (6.6 TB/s), four fifths of it written.  (Block
-// after block in one wavefront, each store behind its own load: 379 us.)
+// after block in one wavefront, each store behind its own load: 379 us.  Values that begin 1 or 3 elements off a multiple of 256: 352 us,
+// 16 elements off: 254 us; quantizing takes the same time at any place.)
 template <bool ROOT, bool NT, bool FULL>
 __device__ __forceinline__ void dequantize_pair(const State8Rec& r, int start, int lane) {
   char* vp = reinterpret_cast<char*>(r.values) + (size_t)start * 4;
