@@ -84,9 +84,18 @@ class TensorList {
   }
   // grad_addresses() if `tensors` holds this list's very objects and no others.
   py::object grad_addresses_in(const py::sequence& tensors, at::ScalarType dtype) const {
-    if ((size_t)PySequence_Size(tensors.ptr()) != t_.size() || !holds(tensors, 0)) return py::none();
+    if (!is_of(tensors)) return py::none();
     return grad_addresses(dtype);
   }
+  // clear_grads() under the same condition; whether it was met
+  bool clear_grads_in(const py::sequence& tensors) {
+    if (!is_of(tensors)) return false;
+    clear_grads();
+    return true;
+  }
+  // Whether `tensors` holds this list's very objects and no others, and `fed` holds them from `first` on.
+  bool rows_of(const py::sequence& tensors, const py::sequence& fed, size_t first) const { return is_of(tensors) && holds(fed, first); }
+  bool is_of(const py::sequence& tensors) const { return (size_t)PySequence_Size(tensors.ptr()) == t_.size() && holds(tensors, 0); }
   // The same for gradients that are given, one for each tensor.
   py::object addresses_of(const py::list& grads, at::ScalarType dtype) const {
     if (grads.size() != t_.size()) return py::none();
@@ -815,10 +824,14 @@ void bind_registry(py::module_& m) {
       .def("addresses_of", [](const TensorList& l, const py::list& grads, const py::object& dtype) {
              return l.addresses_of(grads, torch::python::detail::py_object_to_dtype(dtype));
            }, "grad_addresses for gradients that are given, one for each tensor (None: it has none)")
+      .def("rows_of", &TensorList::rows_of,
+           "whether `tensors` holds the very objects this list was made of and no others, and `fed` holds them from `first` on")
       .def("holds", &TensorList::holds, py::arg("tensors"), py::arg("first") = 0,
            "whether the entries of `tensors` from `first` on are the very objects this list was made of")
       .def("set_grads", &TensorList::set_grads)
-      .def("clear_grads", &TensorList::clear_grads);
+      .def("clear_grads", &TensorList::clear_grads)
+      .def("clear_grads_in", &TensorList::clear_grads_in,
+           "clear_grads if `tensors` is a list or tuple of the very objects this list was made of; whether it is");
 
   py::class_<GradPlan>(m, "GradPlan")
       .def(py::init<std::shared_ptr<TensorList>, std::shared_ptr<TensorList>>(), py::arg("owners"), py::arg("dsts") = nullptr)

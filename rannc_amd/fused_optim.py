@@ -93,11 +93,11 @@ class _Steady:
     __slots__ = ("params", "n", "param_ids", "table", "key", "grad_ptrs", "grad_dtype", "steps_buf", "steps_np", "count", "device",
                  "param_ptr_ends", "fed_by", "numels")
 
-    def same(self, params: List[torch.Tensor], first: int = 0) -> bool:
-        """Whether ``params`` holds the record's very parameters from ``first`` on."""
+    def same(self, params: List[torch.Tensor]) -> bool:
+        """Whether ``params``, which has their number, holds the record's very parameters."""
         if type(self.params) is not tuple:
-            return self.params.holds(params, first)
-        return first + self.n <= len(params) and all(map(is_, self.params, params[first:]))
+            return self.params.holds(params)
+        return all(map(is_, self.params, params))
 
     def addresses(self, grads: List[Optional[torch.Tensor]]) -> Optional[bytes]:
         """Where the parameters' gradients lie; None unless each parameter has one that the table can read, that is also of
@@ -203,14 +203,6 @@ class _FusedBase(torch.optim.Optimizer):
         self._tables.clear()
         self._native_lists.clear()
 
-    def _native_list(self, gi: int, params):
-        """The compiled module's list of a group's parameters: a list may be given other entries in place, so every one is
-        compared (about 1 ns each)."""
-        known = self._native_lists.get(gi)
-        if known is None or len(known) != len(params) or not known.holds(params):
-            known = self._native_lists[gi] = _native.TensorList(params)
-        return known
-
     def _steady_grads(self, gi: int, group) -> Optional["_Steady"]:
         """The group's steady-state record, its table pointing at this step's gradients, or None when anything about
         the group differs from the step that made the record (then the full path runs and makes a new one)."""
@@ -219,11 +211,10 @@ class _FusedBase(torch.optim.Optimizer):
         if st is None or len(params) != st.n:
             return None
         if self._feed is not None and not self._grad_sources:
-            if not st.same(params):
-                return None
             off = self._feed_offsets.get(gi) if self._feed_offsets is not None else None
-            if (off is not None and st.same(self._feed_params, off) and self._feed.held() >= off + st.n and dtype_code(st.grad_dtype) == self._feed.source_dtype()
-                    and (params[0].data_ptr(), params[-1].data_ptr()) == st.param_ptr_ends):
+            # (a feed is the compiled module's, and so is the record's list then)
+            if (off is not None and st.params.rows_of(params, self._feed_params, off) and self._feed.held() >= off + st.n
+                    and dtype_code(st.grad_dtype) == self._feed.source_dtype() and (params[0].data_ptr(), params[-1].data_ptr()) == st.param_ptr_ends):
                 if st.fed_by is not self._feed:
                     self._feed.forget_optim(st.table.handle)      # whatever an earlier table at this address was told
                     st.fed_by = self._feed
@@ -296,7 +287,11 @@ class _FusedBase(torch.optim.Optimizer):
                 for p in params:
                     p.grad = None
                 continue
-            self._native_list(gi, params).clear_grads()
+            # a list may be given other entries in place, so every one is compared (about 1 ns each)
+            known = self._native_lists.get(gi)
+            if known is None or not known.clear_grads_in(params):
+                known = self._native_lists[gi] = _native.TensorList(params)
+                known.clear_grads()
 
     def _scale_source(self, table: _lib.OptimTable) -> _lib.OptimTable:
         """Tell the table where the gradient scale lives, when that changed since its last launch."""
